@@ -1,0 +1,64 @@
+"""The ends of the block operators' ranges, value by value.
+
+Where the other tests compare with a tensor's largest value, these compare every value with its own float64 one, at gates that are
+nearly open or shut and at decays from almost one to almost nothing.  Tolerances count in u = 2^-24.  A gate's logistic function
+is 1 / (1 + 2^t) with t = -x log2(e): rounding t and the constant costs 1.5 |x| u relative, the exponential and
+the reciprocal 6 u, and so it is for 1 minus the gate, which is the function of -x.  softplus is within 8 u, the square root and its
+reciprocal within 4 u, the decay's polynomial within 2 u, and a decay e^l carries l's relative error times |l|.
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+TINY = 2.0**-126  # where float32 begins to lose digits
+
+
+def near(got, want, rel, what, slack=TINY):
+    got, want = got.detach().double().cpu(), want.detach().double().cpu()
+    assert got.shape == want.shape, what
+    err = (got - want).abs()
+    bound = rel.cpu() * want.abs() + slack if torch.is_tensor(rel) else rel * want.abs() + slack
+    worst = torch.where(torch.isfinite(err), err / bound, torch.full_like(err, float("inf"))).flatten().argmax()
+    assert (err <= bound).all(), f"{what}: {got.flatten()[worst]} for {want.flatten()[worst]}, {err.flatten()[worst] / bound.flatten()[worst]} of the bound"
+
+
+def one_step(r, i, lam, x, gh, dt, h0=None):
+    """One step per sequence of the batch, rows of the gates against columns of lam: the operator's and the definition's results.
+    Without an h0 every gradient of x, r and i is a plain product: nothing cancels but what the operator makes cancel."""
+    import tsfast_b200 as b
+
+    D = lam.numel()
+    wide = lambda v: v.to(dt).cuda()[:, None, None].expand(-1, 1, D).contiguous().requires_grad_()  # noqa: E731
+    leaves = [wide(x), wide(r), wide(i), lam.float().cuda().requires_grad_()]
+    state = torch.full((r.numel(), D), 0.0 if h0 is None else h0, device="cuda").requires_grad_()
+    h, last = b.gated_recurrence(*leaves, state)
+    up = wide(gh).detach()
+    got = (h, last, *torch.autograd.grad((h, last), [*leaves, state], (up, torch.zeros_like(last))))
+    x, r, i, lam, state, up = (t.detach().double().requires_grad_() for t in (*leaves, state, up))
+    rho, shut, iota, shut_i = torch.sigmoid(r), torch.sigmoid(-r), torch.sigmoid(i), torch.sigmoid(-i)
+    sp = torch.nn.functional.softplus(lam, threshold=700)
+    l = -8 * sp * rho
+    a, beta = torch.exp(l), torch.sqrt(-torch.expm1(2 * l))
+    before = state[:, None]
+    gl = up * (a * before - a * a / beta * iota * x)
+    out = a * before + beta * iota * x
+    return got, dict(h=out, last=out[:, 0], gx=up * beta * iota, gr=gl * l * shut, gi=up * beta * iota * x * shut_i,
+                     glam=(gl * -8 * rho * torch.sigmoid(lam)).sum((0, 1)), gh0=(up * a)[:, 0], l=l, r=r, i=i, lam=lam)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+def test_gradient_of_r_at_every_gate_and_rate(dt):
+    """gr has the factors l and 1 - rho.  The rates go down to where c softplus(lam) is subnormal and to nothing; sums of relative
+    errors: 1.5 |r| u for rho and for 1 - rho, of which only one is not next to 1, half of it again for beta, and the constants above."""
+    r = torch.tensor([-60.0, -20, -8, -2, 0, 2, 5, 8, 10, 12, 14, 15, 16, 18, 20, 40, 60])
+    lam = torch.tensor([-120.0, -104, -103, -100, -95, -92, -91, -90, -60, -20, -8, -5, -2.5])
+    got, want = one_step(r, torch.zeros_like(r), lam, torch.ones_like(r), torch.ones_like(r), dt)
+    rel = (2.5 * want["r"].abs() + 64) * U + (0 if dt == torch.float32 else torch.finfo(dt).eps / 2 * (1 + 2.0**-7))
+    # float16 steps by 2^-24 below 2^-14.  beta loses digits where beta^2 comes near the smallest normal number: gr's values there
+    # are about beta / 2, 1e-19 and less
+    slack = 2.0**-62 if dt != torch.float16 else 2.0**-25
+    near(got[3], want["gr"].expand_as(got[3]), rel, "gr", slack)
+    assert all(torch.isfinite(t).all() for t in got)

@@ -131,6 +131,12 @@ __device__ __forceinline__ Pair sigmoid2(const Constants& k, Pair x) {
     const float2 d = pair2(add2(bits2(make_float2(ex2(t.x), ex2(t.y))), k.one));
     return bits2(make_float2(rcp(d.x), rcp(d.y)));
 }
+// 1 - s of s = sigmoid(x), as e^-x s: the difference keeps nothing of it where the gate is open (at x = 10 it is 4.5e-5, and s is
+// known to 2^-24). The limit keeps infinity times zero away where s has gone to zero.
+__device__ __forceinline__ Pair complement2(const Constants& k, Pair x, Pair s) {
+    const float2 t = pair2(mul2(x, k.nlog2e));
+    return mul2(bits2(make_float2(ex2(fminf(t.x, 126.f)), ex2(fminf(t.y, 126.f)))), s);
+}
 // 2^l - 1 for l <= 0, of two values. SLOW: l >= -1/2 is known, and the polynomial is all it takes. Else its integer part
 // goes to the exponent; below -115 the result is -1 to the last bit. A NaN passes through.
 template <bool SLOW>
@@ -656,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
 #pragma unroll
         for (int e = 0; e < NP; ++e) {
             const float2 sp = pair2(nsp[e]);
-            per_sp[e] = bits2(make_float2(sp.x < 0.f ? 1.f / sp.x : 0.f, sp.y < 0.f ? 1.f / sp.y : 0.f));  // rho = l per_sp
+            per_sp[e] = bits2(make_float2(1.f / fminf(sp.x, -1.17549435e-38f), 1.f / fminf(sp.y, -1.17549435e-38f)));  // rho = l per_sp
         }
         const int row_bytes = min(Lanes<NP>::chans, p.D - ct * Lanes<NP>::chans) * (int)sizeof(T);
         const unsigned char* src[4];
@@ -750,19 +756,19 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
 #pragma unroll
             for (int j = TS - 1; j >= 0; --j) {
                 if (j < left) {
-                    Pair gh[NP], gx[NP], gr[NP], gi[NP];
-                    read(stage, 0, row0, j, x), read(stage, 3, row0, j, gh);
+                    Pair r[NP], gh[NP], gx[NP], gr[NP], gi[NP];
+                    read(stage, 0, row0, j, x), read(stage, 1, row0, j, r), read(stage, 3, row0, j, gh);
 #pragma unroll
                     for (int e = 0; e < NP; ++e) {
                         const Pair t = add2(gh[e], g[e]);
                         g[e] = mul2(f.a[j][e], t);
-                        const Pair y = mul2(t, f.iota[j][e]), yx = mul2(y, x[e]), l = mul2(f.kappa[j][e], f.beta[j][e]);
-                        gx[e] = mul2(y, f.beta[j][e]);
+                        gx[e] = mul2(mul2(t, f.iota[j][e]), f.beta[j][e]);
                         gi[e] = mul2(mul2(gx[e], x[e]), fma2(f.iota[j][e], k.neg1, k.one));
-                        const Pair ak = mul2(f.a[j][e], mul2(f.kappa[j][e], k.neg1));
-                        const Pair w = mul2(f.a[j][e], fma2(ak, yx, mul2(mul2(l, t), before[j][e])));
+                        // w = l (a g~ h' - (a^2 / beta) g~ iota x) = a g~ kappa (beta h' - a iota x)
+                        const Pair own = mul2(mul2(f.a[j][e], f.iota[j][e]), x[e]);
+                        const Pair w = mul2(mul2(g[e], f.kappa[j][e]), fma2(own, k.neg1, mul2(f.beta[j][e], before[j][e])));
                         wsum[e] = add2(wsum[e], w);
-                        gr[e] = mul2(w, fma2(mul2(l, per_sp[e]), k.neg1, k.one));
+                        gr[e] = mul2(w, complement2(k, r[e], mul2(mul2(f.kappa[j][e], f.beta[j][e]), per_sp[e])));
                     }
                     store_lane<T, NP>(static_cast<T*>(p.out[0]) + o, gx, !MIS || p.whole, n);
                     store_lane<T, NP>(static_cast<T*>(p.out[1]) + o, gr, !MIS || p.whole, n);
