@@ -62,3 +62,12 @@ def test_gradient_of_r_at_every_gate_and_rate(dt):
     slack = 2.0**-62 if dt != torch.float16 else 2.0**-25
     near(got[3], want["gr"].expand_as(got[3]), rel, "gr", slack)
     assert all(torch.isfinite(t).all() for t in got)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_gradient_of_i_at_every_gate(dt):
+    """gi has the factor 1 - iota: the relative error is the gates' (1.5 |i| u, once) and that of the constants."""
+    i = torch.tensor([-60.0, -20, -8, -2, 0, 2, 5, 8, 10, 12, 14, 15, 16, 18, 20, 40, 60])
+    got, want = one_step(torch.zeros_like(i), i, torch.tensor([-20.0, -8, -5, -2.5]), torch.ones_like(i), torch.ones_like(i), dt)
+    rel = (2 * want["i"].abs() + 64) * U + (0 if dt == torch.float32 else torch.finfo(dt).eps / 2 * (1 + 2.0**-7))
+    near(got[4], want["gi"].expand_as(got[4]), rel, "gi")

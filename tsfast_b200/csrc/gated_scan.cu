@@ -137,6 +137,12 @@ __device__ __forceinline__ Pair complement2(const Constants& k, Pair x, Pair s) 
     const float2 t = pair2(mul2(x, k.nlog2e));
     return mul2(bits2(make_float2(ex2(fminf(t.x, 126.f)), ex2(fminf(t.y, 126.f)))), s);
 }
+// The same where s is not at hand, as the function of -x
+__device__ __forceinline__ Pair co_sigmoid2(const Constants& k, Pair x) {
+    const float2 t = pair2(mul2(x, k.nlog2e));
+    const float2 d = pair2(add2(bits2(make_float2(ex2(-t.x), ex2(-t.y))), k.one));
+    return bits2(make_float2(rcp(d.x), rcp(d.y)));
+}
 // 2^l - 1 for l <= 0, of two values. SLOW: l >= -1/2 is known, and the polynomial is all it takes. Else its integer part
 // goes to the exponent; below -115 the result is -1 to the last bit. A NaN passes through.
 template <bool SLOW>
@@ -687,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
                              MIS ? (uint32_t)(reinterpret_cast<uintptr_t>(src[q]) + (row0 + j) * step[q]) : 0u, v);
         };
         struct Coeffs {
-            Pair a[TS][NP], iota[TS][NP], beta[TS][NP], kappa[TS][NP];  // kappa = l / beta
+            Pair a[TS][NP], l[TS][NP], b[TS][NP], m[TS][NP];  // b = beta iota, m = -(a l / beta) iota
         };
         const Pair minus2 = resident(-2.f), tiny = resident(1e-37f);
         int stage = 0;
@@ -711,11 +717,12 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
                         const Pair q = fma2(u, fma2(u, k.neg1, minus2), tiny);
                         const float2 b2 = pair2(q);
                         const Pair s = bits2(make_float2(rsq(b2.x), rsq(b2.y)));
-                        f.iota[j][e] = sigmoid2(k, i[e]);
+                        const Pair si = mul2(s, sigmoid2(k, i[e]));
+                        f.l[j][e] = l;
                         f.a[j][e] = add2(u, k.one);
-                        f.beta[j][e] = mul2(q, s);
-                        f.kappa[j][e] = mul2(l, s);
-                        Pair b = mul2(mul2(f.beta[j][e], f.iota[j][e]), x[e]);
+                        f.b[j][e] = mul2(q, si);
+                        f.m[j][e] = mul2(mul2(f.a[j][e], mul2(l, k.neg1)), si);
+                        Pair b = mul2(f.b[j][e], x[e]);
                         if (!whole && j >= left) f.a[j][e] = k.one, b = 0;
                         H[e] = fma2(f.a[j][e], H[e], b);
                         A[e] = mul2(A[e], f.a[j][e]);
@@ -750,25 +757,23 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
             for (int j = 0; j + 1 < TS; ++j) {
                 read(stage, 0, row0, j, x);
 #pragma unroll
-                for (int e = 0; e < NP; ++e) before[j + 1][e] = fma2(f.a[j][e], before[j][e], mul2(mul2(f.beta[j][e], f.iota[j][e]), x[e]));
+                for (int e = 0; e < NP; ++e) before[j + 1][e] = fma2(f.a[j][e], before[j][e], mul2(f.b[j][e], x[e]));
             }
             long long o = (ch.row0 + row0 + TS - 1) * p.D + d;
 #pragma unroll
             for (int j = TS - 1; j >= 0; --j) {
                 if (j < left) {
-                    Pair r[NP], gh[NP], gx[NP], gr[NP], gi[NP];
-                    read(stage, 0, row0, j, x), read(stage, 1, row0, j, r), read(stage, 3, row0, j, gh);
+                    Pair r[NP], i[NP], gh[NP], gx[NP], gr[NP], gi[NP];
+                    read(stage, 0, row0, j, x), read(stage, 1, row0, j, r), read(stage, 2, row0, j, i), read(stage, 3, row0, j, gh);
 #pragma unroll
                     for (int e = 0; e < NP; ++e) {
                         const Pair t = add2(gh[e], g[e]);
                         g[e] = mul2(f.a[j][e], t);
-                        gx[e] = mul2(mul2(t, f.iota[j][e]), f.beta[j][e]);
-                        gi[e] = mul2(mul2(gx[e], x[e]), fma2(f.iota[j][e], k.neg1, k.one));
-                        // w = l (a g~ h' - (a^2 / beta) g~ iota x) = a g~ kappa (beta h' - a iota x)
-                        const Pair own = mul2(mul2(f.a[j][e], f.iota[j][e]), x[e]);
-                        const Pair w = mul2(mul2(g[e], f.kappa[j][e]), fma2(own, k.neg1, mul2(f.beta[j][e], before[j][e])));
+                        gx[e] = mul2(t, f.b[j][e]);
+                        gi[e] = mul2(mul2(gx[e], x[e]), co_sigmoid2(k, i[e]));
+                        const Pair w = mul2(g[e], fma2(f.m[j][e], x[e], mul2(f.l[j][e], before[j][e])));
                         wsum[e] = add2(wsum[e], w);
-                        gr[e] = mul2(w, complement2(k, r[e], mul2(mul2(f.kappa[j][e], f.beta[j][e]), per_sp[e])));
+                        gr[e] = mul2(w, complement2(k, r[e], mul2(f.l[j][e], per_sp[e])));
                     }
                     store_lane<T, NP>(static_cast<T*>(p.out[0]) + o, gx, !MIS || p.whole, n);
                     store_lane<T, NP>(static_cast<T*>(p.out[1]) + o, gr, !MIS || p.whole, n);
