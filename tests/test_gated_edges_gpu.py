@@ -71,3 +71,12 @@ def test_gradient_of_i_at_every_gate(dt):
     got, want = one_step(torch.zeros_like(i), i, torch.tensor([-20.0, -8, -5, -2.5]), torch.ones_like(i), torch.ones_like(i), dt)
     rel = (2 * want["i"].abs() + 64) * U + (0 if dt == torch.float32 else torch.finfo(dt).eps / 2 * (1 + 2.0**-7))
     near(got[4], want["gi"].expand_as(got[4]), rel, "gi")
+
+
+def test_gradient_of_lam_where_its_sigmoid_and_softplus_end():
+    """glam is a sum times sigmoid(lam) / softplus(lam), which tends to 1. A large state brings the gradient of a channel that
+    hardly decays into sight: c softplus(lam) is subnormal from lam = -85.3 on, with 10 bits left at -96, so 2^-10."""
+    r = torch.tensor([-1.0, 0, 1, 2])
+    lam = torch.tensor([-96.0, -92, -90, -89, -88.5, -87, -80, -30, -17.5, -16.5, -10, -5])
+    got, want = one_step(r, torch.zeros_like(r), lam, torch.zeros_like(r), torch.ones_like(r), torch.float32, 1e15)
+    near(got[5], want["glam"], torch.where(want["lam"] < -85, 2.0**-10, 512 * U), "glam")

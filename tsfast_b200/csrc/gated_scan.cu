@@ -822,9 +822,9 @@ __global__ void __launch_bounds__(1024) gated_lam_kernel(const float* __restrict
         s = 0.f;
         for (int j = 0; j < 32; ++j) s += red[j][dl];
         if (last) {
-            // sigmoid(lam) / softplus(lam) tends to 1 where both underflow
-            const float v = lam[d], sp = softplus(v), sg = 1.f / (1.f + expf(-v));
-            out[d] = s * (sp > 0.f ? sg / sp : 1.f);
+            // sigmoid(lam) / softplus(lam) is 1 - e^lam / 2 and less: one to the last bit below -17, where either underflows later on
+            const float v = lam[d];
+            out[d] = s * (v < -17.f ? 1.f : 1.f / (1.f + expf(-v)) / softplus(v));
         } else {
             out[(long long)blockIdx.y * D + d] = s;
         }
