@@ -80,3 +80,66 @@ def test_gradient_of_lam_where_its_sigmoid_and_softplus_end():
     lam = torch.tensor([-96.0, -92, -90, -89, -88.5, -87, -80, -30, -17.5, -16.5, -10, -5])
     got, want = one_step(r, torch.zeros_like(r), lam, torch.zeros_like(r), torch.ones_like(r), torch.float32, 1e15)
     near(got[5], want["glam"], torch.where(want["lam"] < -85, 2.0**-10, 512 * U), "glam")
+
+
+def decays():
+    r = torch.tensor([-30.0, -10, -4, -1, 0, 0.5, 1, 2, 4, 8, 30])
+    lam = torch.tensor([-30.0, -8, -4, -2, -1, 0, 0.5, 1, 1.5, 2, 3, 4, 6, 8, 10, 12, 20, 60, 300])
+    return r, lam
+
+
+def decay_bound(want):
+    """The relative error of e^l: |l| times l's own (the gate's and softplus's), and a few u for the exponential."""
+    return want["l"].abs() * (1.5 * want["r"].abs() + 20) * U + 8 * U
+
+
+def test_decays_of_every_size():
+    """A state and no input: h is the decay, and so is the gradient of h0, down to where float32 ends."""
+    r, lam = decays()
+    got, want = one_step(r, torch.zeros_like(r), lam, torch.zeros_like(r), torch.ones_like(r), torch.float32, 1.0)
+    bound = decay_bound(want)
+    near(got[0], want["h"].expand_as(got[0]), bound, "h")
+    near(got[1], want["last"], bound[:, 0], "last")
+    near(got[6], want["gh0"], bound[:, 0], "gh0")
+
+
+def test_decays_of_every_size_in_a_step():
+    import tsfast_b200 as b
+
+    r, lam = decays()
+    _, want = one_step(r, torch.zeros_like(r), lam, torch.zeros_like(r), torch.ones_like(r), torch.float32, 1.0)
+    rows = r.cuda()[:, None].expand(-1, lam.numel()).contiguous()
+    state = torch.ones_like(rows)
+    h = b.gated_recurrence_step(torch.zeros_like(rows), rows, rows, lam.cuda(), state)
+    near(h, want["last"], decay_bound(want)[:, 0], "h")
+    assert torch.equal(h, state)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_layers_that_forget(packed):
+    """Decays from 0.999 down to 1e-4 in one warp of channels, and no value that cancels: every term is positive, so every state is
+    within the sum of its steps' errors. The same for the adjoint's carry (gh0) of a positive upstream gradient."""
+    import tsfast_b200 as b
+    from test_gated_gpu import definition
+
+    L, D = 61, 96
+    g = torch.Generator(device="cuda").manual_seed(11)
+    rand = lambda *s: torch.rand(*s, device="cuda", generator=g)  # noqa: E731
+    base = torch.logspace(-4, -0.0004345, D, device="cuda", dtype=torch.float64)
+    lam = torch.log(torch.expm1(-torch.log(base) / 8)).float().requires_grad_()
+    x, r, i = (rand(L, D).requires_grad_(), (6 * rand(L, D) - 3).requires_grad_(), (6 * rand(L, D) - 3).requires_grad_())
+    h0, gh, gl = (10 + rand(1, D)).requires_grad_(), torch.zeros(L, D, device="cuda"), rand(1, D)
+    gh[20:] = rand(L - 20, D)
+    if packed:
+        h, last = b.gated_recurrence(x, r, i, lam, h0, cu_seqlens=torch.tensor([0, L], device="cuda"))
+    else:
+        h, last = (t[0] if k == 0 else t for k, t in enumerate(b.gated_recurrence(x[None], r[None], i[None], lam, h0)))
+    gh0 = torch.autograd.grad((h, last), h0, (gh, gl))[0]
+    want, want_last, *grads = definition(x, r, i, lam, h0, [0, L], 8.0, gh, gl)
+    # a step's decay has |l| (1.5 * 3 + 20) u + 8 u, |l| up to 9.3 * 0.96, that is 220 u where the decay is about 1e-4 and the
+    # state forgets the step at once; what is remembered for long has |l| below 1: at most 33 u a step, 61 steps, and 220 u for one more
+    near(h, want, (61 * 33 + 220) * U, "h")
+    near(last, want_last, (61 * 33 + 220) * U, "last")
+    # gh0 is a product of twenty decays and more: the sum of their |l| counts, l's error alone being (4.5 + 20) u of it
+    total = (8 * torch.nn.functional.softplus(lam.detach().double()) * torch.sigmoid(r.detach().double())[:21].sum(0))[None]
+    near(gh0, grads[4], (total * 25 + 21 * 8 + 61 * 33 + 220) * U, "gh0")

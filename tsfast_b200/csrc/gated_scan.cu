@@ -7,9 +7,9 @@
 // (w is the gradient of l times l: both l's derivatives, by r and by lam, are l times something, and l / beta stays
 // finite where beta goes to zero); and the form for one token per row against a cache of states.
 //
-// Numerics: u = e^l - 1 is computed to full relative accuracy (to base 2: the integer part goes to the exponent, the rest
-// through a polynomial fitted to the smallest largest relative error by Lawson's iteration), so a = 1 + u and beta^2 = -u (2 + u) are
-// both right where a is close to 1, which is where such a layer works. The state, the gates, all products and all
+// Numerics: u = e^l - 1 and a are both computed to full relative accuracy (to base 2: the integer part goes to the exponent, the rest
+// through a polynomial fitted to the smallest largest relative error by Lawson's iteration), so a and beta^2 = -u (2 + u) are
+// right where a is close to 1, which is where such a layer works, and where it is small. The state, the gates, all products and all
 // sums are float32; sequences are rounded once, when they are stored. The adjoint recomputes the states from
 // float32 states kept at every tile instead of reading the rounded h back: one tensor less to read, and no error
 // of 2^-9 in h_{t-1}.
@@ -143,14 +143,18 @@ __device__ __forceinline__ Pair co_sigmoid2(const Constants& k, Pair x) {
     const float2 d = pair2(add2(bits2(make_float2(ex2(-t.x), ex2(-t.y))), k.one));
     return bits2(make_float2(rcp(d.x), rcp(d.y)));
 }
-// 2^l - 1 for l <= 0, of two values. SLOW: l >= -1/2 is known, and the polynomial is all it takes. Else its integer part
-// goes to the exponent; below -115 the result is -1 to the last bit. A NaN passes through.
+// Of two l <= 0: u = 2^l - 1 and a = 2^l, each to the last bits (a - 1 keeps nothing of u where a is close to one, and u + 1
+// nothing of a where a is small). SLOW: l >= -1/2 is known, and the polynomial is all it takes. Else its integer part
+// goes to the exponent; a below 2^-126 is given as 2^-126. A NaN passes through.
+struct Decay {
+    Pair u, a;
+};
 template <bool SLOW>
-__device__ __forceinline__ Pair exp2m1_neg2(const Constants& k, Pair l2) {
+__device__ __forceinline__ Decay decay2(const Constants& k, Pair l2) {
     Pair f = l2, s = 0;
     if constexpr (!SLOW) {
         const float2 c = pair2(l2);
-        l2 = bits2(make_float2(max_nan(c.x, -115.f), max_nan(c.y, -115.f)));
+        l2 = bits2(make_float2(max_nan(c.x, -126.f), max_nan(c.y, -126.f)));
         const Pair t = add2(l2, bits2(both(12582912.f)));  // 1.5 * 2^23 + l: the low bits hold round(l)
         f = fma2(add2(t, bits2(both(-12582912.f))), k.neg1, l2);
         const float2 i = pair2(t);
@@ -162,7 +166,8 @@ __device__ __forceinline__ Pair exp2m1_neg2(const Constants& k, Pair l2) {
     q = fma2(q, f, k.c[1]);
     q = fma2(q, f, k.c[0]);
     q = mul2(f, q);
-    return SLOW ? q : fma2(s, q, add2(s, k.neg1));
+    if constexpr (SLOW) return {q, add2(q, k.one)};
+    else return {fma2(s, q, add2(s, k.neg1)), fma2(s, q, s)};
 }
 // u = a - 1: -beta^2 = u (2 + u)
 __device__ __forceinline__ Pair minus_beta2(Pair u) { return fma2(u, u, add2(u, u)); }
@@ -529,9 +534,9 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const Args p) {
                     read(0, x), read(1, r), read(2, i);
 #pragma unroll
                     for (int e = 0; e < NP; ++e) {
-                        const Pair u = exp2m1_neg2<decltype(slow)::value>(k, mul2(nsp2[e], sigmoid2(k, r[e])));
-                        const float2 q = pair2(minus_beta2(u));
-                        a[j][e] = add2(u, k.one);
+                        const Decay dec = decay2<decltype(slow)::value>(k, mul2(nsp2[e], sigmoid2(k, r[e])));
+                        const float2 q = pair2(minus_beta2(dec.u));
+                        a[j][e] = dec.a;
                         b[j][e] = mul2(mul2(bits2(make_float2(root(-q.x), root(-q.y))), x[e]), sigmoid2(k, i[e]));
                         if (!whole && j >= left) a[j][e] = k.one, b[j][e] = 0;
                         m[e].sum = fma2(a[j][e], m[e].sum, b[j][e]);
@@ -712,16 +717,16 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
 #pragma unroll
                     for (int e = 0; e < NP; ++e) {
                         const Pair rho = sigmoid2(k, r[e]), l = mul2(nsp[e], rho);
-                        const Pair u = exp2m1_neg2<decltype(slow)::value>(k, mul2(nsp2[e], rho));
+                        const auto [u, a] = decay2<decltype(slow)::value>(k, mul2(nsp2[e], rho));
                         // beta^2 and a little, so that l / beta is 0 where l is
                         const Pair q = fma2(u, fma2(u, k.neg1, minus2), tiny);
                         const float2 b2 = pair2(q);
                         const Pair s = bits2(make_float2(rsq(b2.x), rsq(b2.y)));
                         const Pair si = mul2(s, sigmoid2(k, i[e]));
                         f.l[j][e] = l;
-                        f.a[j][e] = add2(u, k.one);
+                        f.a[j][e] = a;
                         f.b[j][e] = mul2(q, si);
-                        f.m[j][e] = mul2(mul2(f.a[j][e], mul2(l, k.neg1)), si);
+                        f.m[j][e] = mul2(mul2(a, mul2(l, k.neg1)), si);
                         Pair b = mul2(f.b[j][e], x[e]);
                         if (!whole && j >= left) f.a[j][e] = k.one, b = 0;
                         H[e] = fma2(f.a[j][e], H[e], b);
@@ -921,10 +926,10 @@ __global__ void __launch_bounds__(kStepThreads) gated_step_kernel(const StepArgs
     for (long long row = b;;) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const Pair u = exp2m1_neg2<false>(k, mul2(nsp2[e], sigmoid2(k, r[e])));
+            const auto [u, a] = decay2<false>(k, mul2(nsp2[e], sigmoid2(k, r[e])));
             const float2 q = pair2(minus_beta2(u));
             const Pair beta = bits2(make_float2(root(-q.x), root(-q.y)));
-            h[e] = fma2(add2(u, k.one), h[e], mul2(mul2(beta, sigmoid2(k, i[e])), x[e]));
+            h[e] = fma2(a, h[e], mul2(mul2(beta, sigmoid2(k, i[e])), x[e]));
         }
         const Pair y[2] = {have ? h[0] : 0, have ? h[1] : 0};
         T* out = static_cast<T*>(p.out) + row * p.D + d;
