@@ -143,3 +143,14 @@ def test_layers_that_forget(packed):
     # gh0 is a product of twenty decays and more: the sum of their |l| counts, l's error alone being (4.5 + 20) u of it
     total = (8 * torch.nn.functional.softplus(lam.detach().double()) * torch.sigmoid(r.detach().double())[:21].sum(0))[None]
     near(gh0, grads[4], (total * 25 + 21 * 8 + 61 * 33 + 220) * U, "gh0")
+
+
+def test_channels_that_hardly_change():
+    """beta = sqrt(1 - a^2) of a channel with a rate near the end of float32: beta^2 may lose the smallest normal number, 2^-126,
+    and beta half of that relative to beta^2 (1.6e-34 at lam = -79, that is 4e-5)."""
+    r = torch.tensor([-1.0, 0, 1])
+    lam = torch.tensor([-79.0, -75, -70, -60])
+    got, want = one_step(r, torch.zeros_like(r), lam, torch.ones_like(r), torch.ones_like(r), torch.float32)
+    beta2 = -torch.expm1(2 * want["l"])
+    near(got[2], want["gx"].expand_as(got[2]), 72 * U + TINY / beta2 / 2, "gx")
+    near(got[0], want["h"].expand_as(got[0]), 72 * U, "h")

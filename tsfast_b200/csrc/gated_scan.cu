@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
         struct Coeffs {
             Pair a[TS][NP], l[TS][NP], b[TS][NP], m[TS][NP];  // b = beta iota, m = -(a l / beta) iota
         };
-        const Pair minus2 = resident(-2.f), tiny = resident(1e-37f);
+        const Pair minus2 = resident(-2.f), tiny = resident(1.17549435e-38f);
         int stage = 0;
         auto gates = [&](int s, Coeffs& f) {
             const int row0 = first_row(s), left = row0 < 0 ? 0 : ch.len - row0;
@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
                     for (int e = 0; e < NP; ++e) {
                         const Pair rho = sigmoid2(k, r[e]), l = mul2(nsp[e], rho);
                         const auto [u, a] = decay2<decltype(slow)::value>(k, mul2(nsp2[e], rho));
-                        // beta^2 and a little, so that l / beta is 0 where l is
+                        // beta^2 and the smallest normal number, so that l / beta is 0 where l is
                         const Pair q = fma2(u, fma2(u, k.neg1, minus2), tiny);
                         const float2 b2 = pair2(q);
                         const Pair s = bits2(make_float2(rsq(b2.x), rsq(b2.y)));
