@@ -174,7 +174,10 @@ __global__ void __launch_bounds__(256) quant_weight_kernel(const T* __restrict__
     const int n0 = blockIdx.y * kBlock, k = blockIdx.x * kBlock + (threadIdx.x & 127), half = threadIdx.x >> 7;
     float m = 0.f;
     for (int r = half; r < kBlock; r += 2)
-        if (n0 + r < N && k < K) m = fmaxf(m, fabsf(to_float(w[(long long)(n0 + r) * ldw + k])));
+        if (n0 + r < N && k < K) {
+            const float v = fabsf(to_float(w[(long long)(n0 + r) * ldw + k]));
+            if (v <= 3.402823466e38f) m = fmaxf(m, v);  // what is not finite is lost itself, and sets no scale
+        }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
     if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = m;
