@@ -1,0 +1,136 @@
+"""What the block operators' host path does beside a plain eager call: calls that are recorded or interpreted (a tracer, a
+dispatch mode, fake tensors), derivatives that do not exist, tensors of inference mode, constants that float32 does not hold.
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def tensors(dt=torch.float32, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x, r, i = (torch.randn(2, 37, 24, device="cuda", generator=g).to(dt) for _ in range(3))
+    lam = torch.randn(24, device="cuda", generator=g) - 3
+    w = torch.rand(24, device="cuda", generator=g).to(dt) + 0.5
+    return x, r, i, lam, w
+
+
+def calls(q=None):
+    """Every operator as a function of (x, r, i, lam, w), tensors of [2, 37, 24]."""
+    import tsfast_b200 as b
+
+    q = q or b.quantize_weight(torch.randn(40, 24, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)))
+    cu = torch.tensor([0, 30, 74], device="cuda")
+
+    def step(x, r, i, lam, w):
+        state = torch.ones(37, 24, device="cuda") * lam
+        return b.gated_recurrence_step(x[0], r[0], i[0], lam, state), state
+
+    return {"recurrence": lambda x, r, i, lam, w: b.gated_recurrence(x, r, i, lam),
+            "recurrence 4-d": lambda x, r, i, lam, w: b.gated_recurrence(x[None], r[None], i[None], lam, lam.expand(1, 2, 24)),
+            "recurrence packed": lambda x, r, i, lam, w: b.gated_recurrence(x.reshape(74, 24), r.reshape(74, 24), i.reshape(74, 24), lam, cu_seqlens=cu),
+            "step": step,
+            "gated_norm": lambda x, r, i, lam, w: b.gated_norm(x, r, w),
+            "residual_norm": lambda x, r, i, lam, w: b.residual_norm(x, i, w, gate=r, scale=w),
+            "quant_linear": lambda x, r, i, lam, w: b.quant_linear(x.half(), *q),
+            "quantize_weight": lambda x, r, i, lam, w: tuple(t.float() for t in b.quantize_weight(x[0]))}
+
+
+NAMES = ["recurrence", "recurrence 4-d", "recurrence packed", "step", "gated_norm", "residual_norm", "quant_linear", "quantize_weight"]
+
+
+def flat(out):
+    return [out] if torch.is_tensor(out) else list(out)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_traced_call_runs_the_operator(name):
+    f = calls()[name]
+    with torch.no_grad():
+        traced = torch.jit.trace(f, tensors(), check_trace=False)
+        assert "b200scan::" in str(traced.graph)
+        for seed in (0, 5):
+            args = tensors(seed=seed)
+            junk = [torch.full((2, 37, 24), 7.0, device="cuda") for _ in range(8)]  # what an uninitialised result would show
+            del junk
+            for a, w in zip(flat(traced(*args)), flat(f(*args)), strict=True):
+                assert torch.equal(a, w)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_dispatch_mode_sees_the_call(name):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    seen, f, args = [], calls()[name], tensors()
+    with torch.no_grad():
+        want = f(*args)
+        with Log():
+            got = f(*args)
+    assert any(s.startswith("b200scan") for s in seen), seen
+    assert all(torch.equal(a, w) for a, w in zip(flat(got), flat(want), strict=True))
+
+
+def test_gradients_under_a_dispatch_mode():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Pass(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    for name in ("recurrence", "gated_norm", "residual_norm"):
+        f = calls()[name]
+
+        def grads():
+            leaves = [t.requires_grad_() for t in tensors()]
+            return torch.autograd.grad(sum(o.square().sum() for o in flat(f(*leaves))), leaves, allow_unused=True, materialize_grads=True)
+
+        want = grads()
+        with Pass():
+            got = grads()
+        assert all(torch.equal(a, w) for a, w in zip(got, want, strict=True))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_make_fx_records_the_operator(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    f, args = calls()[name], tensors()
+    with torch.no_grad():
+        module = make_fx(f)(*args)
+        assert "b200scan" in module.code
+        for a, w in zip(flat(module(*args)), flat(f(*args)), strict=True):
+            assert torch.equal(a, w)
+
+
+def test_fake_tensors_give_fake_results():
+    import tsfast_b200 as b
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode(), torch.no_grad():
+        x, lam, w = torch.empty(2, 37, 24, device="cuda"), torch.empty(24, device="cuda"), torch.empty(24, device="cuda")
+        h, last = b.gated_recurrence(x, x, x, lam)
+        assert h.shape == x.shape and last.shape == (2, 24) and last.dtype == torch.float32
+        h, last = b.gated_recurrence(x[:, :0], x[:, :0], x[:, :0], lam)
+        assert h.shape == (2, 0, 24)
+        h, last = b.gated_recurrence(x[None, :, :0], x[None, :, :0], x[None, :, :0], lam)
+        assert h.shape == (1, 2, 0, 24) and last.shape == (1, 2, 24)
+        assert b.gated_recurrence_step(x[0], x[0], x[0], lam, torch.empty(50, 24, device="cuda")).shape == (37, 24)
+        assert b.gated_norm(x, x, w).shape == x.shape
+        y, r = b.residual_norm(x, x, w)
+        assert y.shape == r.shape == x.shape
+        q, scale = b.quantize_weight(torch.empty(300, 200, device="cuda"))
+        assert q.shape == (300, 200) and q.stride(0) == 256 and scale.shape == (3, 2) and q.dtype == torch.float8_e4m3fn
+        assert b.quant_linear(torch.empty(2, 3, 200, device="cuda").half(), q, scale).shape == (2, 3, 300)
+
+
+def test_opcheck_of_the_weight():
+    from tsfast_b200 import quant_b200
+
+    for shape in ((300, 200), (1, 128)):
+        torch.library.opcheck(quant_b200._weight_op, (torch.randn(*shape, device="cuda"),), test_utils=("test_faketensor",))

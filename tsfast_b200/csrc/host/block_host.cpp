@@ -6,8 +6,10 @@
 // library that _lib.py loaded, whichever that is. Every failure is a C++ exception, which reaches Python as RuntimeError.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -96,6 +98,15 @@ struct Launch {
     }
     void* stream() const { return c10::cuda::getCurrentCUDAStream(index).stream(); }
 };
+
+// Whether somebody has to see the call: a tracer, a dispatch mode, a tensor with a dispatch of its own (a fake one). It is then
+// left to the custom op, which goes through the dispatcher; here only the kernels' plain allocations would be seen.
+bool recorded(std::initializer_list<const Tensor*> operands) {
+    if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::any_modes_set()) return true;
+    for (const Tensor* t : operands)
+        if (t->defined() && t->unsafeGetTensorImpl()->is_python_dispatch()) return true;
+    return false;
+}
 
 Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::empty(sizes, like.options().dtype(type).memory_format(std::nullopt).requires_grad(false)); }
 Tensor workspace(size_t bytes, const Tensor& like) { return empty({(int64_t)std::max<size_t>(bytes, 256)}, at::kByte, like); }
@@ -212,8 +223,11 @@ struct GatedNode : Function<GatedNode> {
     }
 };
 
-std::tuple<Tensor, Tensor> gated_recurrence(Tensor x, Tensor r, Tensor i, const Tensor& lam, Opt h0, const Opt& cu, double c) {
+// The calls of a user, as those below: nothing where the call is to be recorded
+std::optional<std::tuple<Tensor, Tensor>> gated_recurrence(Tensor x, Tensor r, Tensor i, const Tensor& lam, Opt h0, const Opt& cu, double c) {
     const char* op = "gated_recurrence";
+    const Tensor h0_ = get(h0), cu_ = get(cu);
+    if (recorded({&x, &r, &i, &lam, &h0_, &cu_})) return {};
     const bool shaped = !has(cu) && x.dim() != 3;
     std::vector<int64_t> lead;
     if (shaped) {  // any number of leading axes, as one
@@ -246,13 +260,11 @@ std::tuple<Tensor, Tensor> gated_recurrence(Tensor x, Tensor r, Tensor i, const 
         rows.push_back(h.size(1)), rows.push_back(h.size(2)), state.push_back(h.size(2));
         h = h.reshape(rows), last = last.reshape(state);
     }
-    return {h, last};
+    return std::tuple(h, last);
 }
 
 Tensor gated_step(const Tensor& x_, const Tensor& r_, const Tensor& i_, const Tensor& lam_, Tensor state, const Opt& slots_, double c) {
     const char* op = "gated_recurrence_step";
-    if (at::GradMode::is_enabled() && (x_.requires_grad() || r_.requires_grad() || i_.requires_grad() || lam_.requires_grad() || state.requires_grad()))
-        refuse(op, "it has no gradient (call it under torch.no_grad(), or train with gated_recurrence)");
     check_sequences(op, x_, r_, i_, lam_, 2, c);
     const int64_t B = x_.size(0), D = x_.size(1);
     if (state.scalar_type() != at::kFloat || state.device() != x_.device() || state.dim() != 2 || state.size(1) != D)
@@ -277,6 +289,13 @@ Tensor gated_step(const Tensor& x_, const Tensor& r_, const Tensor& i_, const Te
           "b200_gated_step");
     state.unsafeGetTensorImpl()->bump_version();
     return h;
+}
+std::optional<Tensor> gated_recurrence_step(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam, const Tensor& state, const Opt& slots, double c) {
+    if (at::GradMode::is_enabled() && (x.requires_grad() || r.requires_grad() || i.requires_grad() || lam.requires_grad() || state.requires_grad()))
+        refuse("gated_recurrence_step", "it has no gradient (call it under torch.no_grad(), or train with gated_recurrence)");
+    const Tensor at = get(slots);
+    if (recorded({&x, &r, &i, &lam, &state, &at})) return {};
+    return gated_step(x, r, i, lam, state, slots, c);
 }
 
 // ---------------------------------------------------------------------------------------------- block norms
@@ -381,10 +400,12 @@ struct NormNode : Function<NormNode> {
 };
 
 // the whole operator over [..., D]; without a residual the second result is undefined
-std::tuple<Tensor, Opt> block_norm(const char* op, const Tensor& x, const Opt& residual, const Opt& gate, const Opt& w1, const Opt& b1, const Opt& scale,
+std::optional<std::tuple<Tensor, Opt>> block_norm(const char* op, const Tensor& x, const Opt& residual, const Opt& gate, const Opt& w1, const Opt& b1, const Opt& scale,
                                    const Opt& w2, const Opt& b2, int64_t kind, int64_t act, double eps) {
     const Params w = {get(w1), get(b1), get(scale), get(w2), get(b2)};
-    check_norm(op, x, get(residual), get(gate), w, kind, eps);
+    const Tensor residual_ = get(residual), gate_ = get(gate);
+    if (recorded({&x, &residual_, &gate_, &w[0], &w[1], &w[2], &w[3], &w[4]})) return {};
+    check_norm(op, x, residual_, gate_, w, kind, eps);
     const bool flat = x.dim() == 2;
     const int64_t D = x.size(-1);
     auto rows = [&](const Opt& t) -> Opt { return !has(t) ? Opt() : flat ? t : Opt(t->reshape({x.numel() / D, D})); };
@@ -401,14 +422,15 @@ std::tuple<Tensor, Opt> block_norm(const char* op, const Tensor& x, const Opt& r
         y = y.reshape(x.sizes());
         if (r.defined()) r = r.reshape(x.sizes());
     }
-    return {y, r.defined() ? Opt(r) : Opt()};
+    return std::tuple(y, r.defined() ? Opt(r) : Opt());
 }
 
-Tensor gated_norm(const Tensor& x, const Opt& gate, const Opt& weight, const Opt& bias, int64_t kind, int64_t act, double eps) {
+std::optional<Tensor> gated_norm(const Tensor& x, const Opt& gate, const Opt& weight, const Opt& bias, int64_t kind, int64_t act, double eps) {
     if (!has(weight)) refuse("gated_norm", "weight is required");
-    return std::get<0>(block_norm("gated_norm", x, {}, gate, weight, bias, {}, {}, {}, kind, act, eps));
+    const auto out = block_norm("gated_norm", x, {}, gate, weight, bias, {}, {}, {}, kind, act, eps);
+    return out ? std::optional(std::get<0>(*out)) : std::nullopt;
 }
-std::tuple<Tensor, Opt> residual_norm(const Tensor& x, const Opt& residual, const Opt& weight, const Opt& bias, const Opt& gate, const Opt& scale,
+std::optional<std::tuple<Tensor, Opt>> residual_norm(const Tensor& x, const Opt& residual, const Opt& weight, const Opt& bias, const Opt& gate, const Opt& scale,
                                       const Opt& post_weight, const Opt& post_bias, int64_t kind, int64_t act, double eps) {
     if (!has(residual)) refuse("residual_norm", "residual is required");
     if (!has(weight)) refuse("residual_norm", "weight is required");
@@ -420,7 +442,7 @@ std::tuple<Tensor, Opt> residual_norm(const Tensor& x, const Opt& residual, cons
 constexpr int64_t kBlock = 128;
 int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
 
-std::tuple<Tensor, Tensor> quantize_weight(const Tensor& w_) {
+std::tuple<Tensor, Tensor> quant_weight(const Tensor& w_) {
     const char* op = "quantize_weight";
     const int tag = tag_of(w_.scalar_type());
     if (tag < 0 || !w_.is_cuda() || w_.dim() != 2 || w_.numel() == 0)
@@ -434,6 +456,11 @@ std::tuple<Tensor, Tensor> quantize_weight(const Tensor& w_) {
     return {q, scale};
 }
 
+std::optional<std::tuple<Tensor, Tensor>> quantize_weight(const Tensor& w) {
+    if (recorded({&w})) return {};
+    return quant_weight(w);
+}
+
 // where TMA can read it: unit column stride, a row pitch that is a multiple of 16, a 16-byte aligned base; else a copy
 Tensor readable(const Tensor& q) {
     const int64_t N = q.size(0), K = q.size(1);
@@ -443,7 +470,7 @@ Tensor readable(const Tensor& q) {
     return copy;
 }
 
-Tensor quant_linear(const Tensor& x_, const Tensor& q_, const Tensor& scale_, const Opt& bias_) {
+Tensor quant_product(const Tensor& x_, const Tensor& q_, const Tensor& scale_, const Opt& bias_) {
     const char* op = "quant_linear";
     if ((x_.scalar_type() != at::kBFloat16 && x_.scalar_type() != at::kHalf) || !x_.is_cuda() || x_.dim() < 1)
         refuse(op, "x is ", Say{x_}, ", expected bfloat16 or float16 [..., K] in CUDA memory");
@@ -456,8 +483,6 @@ Tensor quant_linear(const Tensor& x_, const Tensor& q_, const Tensor& scale_, co
     if (bias.defined() && ((bias.scalar_type() != x_.scalar_type() && bias.scalar_type() != at::kFloat) || bias.device() != x_.device() || bias.dim() != 1 ||
                            bias.size(0) != N))
         refuse(op, "bias is ", Say{bias}, ", expected [", N, "] of ", name_of(x_.scalar_type()), " or float32 on ", x_.device());
-    if (at::GradMode::is_enabled() && (x_.requires_grad() || scale_.requires_grad() || wants(bias_)))
-        refuse(op, "it has no gradient (call it under torch.no_grad())");
     const int64_t M = x_.numel() / K;
     const bool flat = x_.dim() == 2;
     const Tensor x = unit(flat ? x_ : x_.reshape({M, K})), q = readable(q_), scale = dense(scale_);
@@ -472,6 +497,13 @@ Tensor quant_linear(const Tensor& x_, const Tensor& q_, const Tensor& scale_, co
     shape.back() = N;
     return y.reshape(shape);
 }
+std::optional<Tensor> quant_linear(const Tensor& x, const Tensor& q, const Tensor& scale, const Opt& bias) {
+    if (at::GradMode::is_enabled() && (x.requires_grad() || scale.requires_grad() || wants(bias)))
+        refuse("quant_linear", "it has no gradient (call it under torch.no_grad())");
+    const Tensor b = get(bias);
+    if (recorded({&x, &q, &scale, &b})) return {};
+    return quant_product(x, q, scale, bias);
+}
 
 }  // namespace
 
@@ -481,6 +513,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("gated_recurrence", &gated_recurrence);
     m.def("gated_forward", &gated_forward);
     m.def("gated_backward", &gated_backward);
+    m.def("gated_recurrence_step", &gated_recurrence_step);
     m.def("gated_step", &gated_step);
     m.def("gated_norm", &gated_norm);
     m.def("residual_norm", &residual_norm);
@@ -495,5 +528,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         return norm_backward(get(gy), get(gr), x, get(residual), get(gate), {get(w[0]), get(w[1]), get(w[2]), get(w[3]), get(w[4])}, stats, kind, act, eps);
     });
     m.def("quantize_weight", &quantize_weight);
+    m.def("quant_weight", &quant_weight);
     m.def("quant_linear", &quant_linear);
+    m.def("quant_product", &quant_product);
 }

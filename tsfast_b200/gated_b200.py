@@ -13,11 +13,13 @@ float32 whatever the sequences' type, and sequences may be packed end to end.
 * ``gated_recurrence_step(x, r, i, lam, state, slots=None, c=8.0)`` -> ``h``: one token per row, against a cache of
   float32 states that is updated in place.
 
-Eager calls take the host path in ``csrc/host/block_host.cpp``; the custom ops below are what ``torch.compile`` sees.
-Nothing falls back: what the kernels cannot take raises.
+Eager calls take the host path in ``csrc/host/block_host.cpp``; the custom ops below are what ``torch.compile``, tracers,
+dispatch modes and fake tensors see (the host path returns None for those).  Nothing falls back: what the kernels cannot take raises.
 """
 
 from __future__ import annotations
+
+import math
 
 import torch
 
@@ -91,11 +93,14 @@ def gated_recurrence(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, lam: tor
     and rows before the first and behind the last get zeros, in ``h`` and in the gradients.
     """
     if not torch.compiler.is_compiling():
-        return _lib.host().gated_recurrence(x, r, i, lam, h0, cu_seqlens, c)
+        out = _lib.host().gated_recurrence(x, r, i, lam, h0, cu_seqlens, c)
+        if out is not None:
+            return out
     if cu_seqlens is not None or x.dim() == 3:
         return _gated_op(x, r, i, lam, h0, cu_seqlens, float(c))[:2]
     lead, tail = x.shape[:-2], x.shape[-2:]
-    h, last, _ = _gated_op(*(t.reshape(-1, *tail) for t in (x, r, i)), lam, None if h0 is None else h0.reshape(-1, tail[1]), None, float(c))
+    n = math.prod(lead)
+    h, last, _ = _gated_op(*(t.reshape(n, *tail) for t in (x, r, i)), lam, None if h0 is None else h0.reshape(n, tail[1]), None, float(c))
     return h.reshape(x.shape), last.reshape(*lead, tail[1])
 
 
@@ -118,6 +123,8 @@ def gated_recurrence_step(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, lam
     outside the cache (-1 for an empty row of a padded batch) leaves the cache alone and its row of ``h`` is zeros; rows
     that name the same slot are applied in row order.  There is no gradient: train with ``gated_recurrence``.
     """
-    if torch.compiler.is_compiling():
-        return _step_op(x, r, i, lam, state, slots, float(c))
-    return _lib.host().gated_step(x, r, i, lam, state, slots, c)
+    if not torch.compiler.is_compiling():
+        out = _lib.host().gated_recurrence_step(x, r, i, lam, state, slots, c)
+        if out is not None:
+            return out
+    return _step_op(x, r, i, lam, state, slots, float(c))

@@ -12,7 +12,8 @@ and ``act`` SiLU, the logistic function or one:
 ``glue_b200.layer_norm`` and ``gate_residual`` are the float32 operators of the LRU and S5 blocks up to 512 features; these
 take float32, bfloat16 and float16 rows of up to 8192, sums and statistics in float32, every result rounded once.
 Parameters are of the rows' type or float32.  Eager calls take the host path in ``csrc/host/block_host.cpp``; the custom
-ops below are what ``torch.compile`` sees.  What the kernels cannot take raises.
+ops below are what ``torch.compile``, tracers, dispatch modes and fake tensors see (the host path returns None for those).  What
+the kernels cannot take raises.
 """
 
 from __future__ import annotations
@@ -95,7 +96,7 @@ def _codes(op, kind, activation):
                            "'sigmoid' or None") from None
 
 
-def _compiled(x, residual, gate, params, kind, act, eps):
+def _composed(x, residual, gate, params, kind, act, eps):
     flat = lambda t: None if t is None else t.reshape(-1, x.shape[-1])  # noqa: E731
     y, r, _ = _norm_op(flat(x), flat(residual), flat(gate), *params, kind, act, float(eps))
     return y.reshape(x.shape), r if residual is None else r.reshape(x.shape)
@@ -106,9 +107,11 @@ def gated_norm(x: torch.Tensor, gate: torch.Tensor | None, weight: torch.Tensor,
     """``(n(x) weight + bias) act(gate)`` over the last axis of ``x [..., D]``, ``D <= 8192``; ``gate`` None: no gate.
     ``bias`` goes with ``kind="layer"``.  Differentiable in all tensors; the result is dense."""
     kind, act = _codes("gated_norm", kind, activation)
-    if torch.compiler.is_compiling():
-        return _compiled(x, None, gate, (weight, bias, None, None, None), kind, act, eps)[0]
-    return _lib.host().gated_norm(x, gate, weight, bias, kind, act, eps)
+    if not torch.compiler.is_compiling():
+        out = _lib.host().gated_norm(x, gate, weight, bias, kind, act, eps)
+        if out is not None:
+            return out
+    return _composed(x, None, gate, (weight, bias, None, None, None), kind, act, eps)[0]
 
 
 def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -121,6 +124,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     ``[D]``.  Without ``post_weight`` x enters as it is, without ``gate`` or ``scale`` they are one; the norm reads the
     unrounded ``r``.  Differentiable in all tensors, with gradients through both results."""
     kind, act = _codes("residual_norm", kind, activation)
-    if torch.compiler.is_compiling():
-        return _compiled(x, residual, gate, (post_weight, post_bias, scale, weight, bias), kind, act, eps)
-    return _lib.host().residual_norm(x, residual, weight, bias, gate, scale, post_weight, post_bias, kind, act, eps)
+    if not torch.compiler.is_compiling():
+        out = _lib.host().residual_norm(x, residual, weight, bias, gate, scale, post_weight, post_bias, kind, act, eps)
+        if out is not None:
+            return out
+    return _composed(x, residual, gate, (post_weight, post_bias, scale, weight, bias), kind, act, eps)

@@ -24,12 +24,28 @@ __all__ = ["quantize_weight", "quant_linear"]
 def quantize_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(q, scale)`` of a weight ``[N, K]`` (float32, bfloat16 or float16): ``q`` float8_e4m3fn ``[N, K]`` with a row pitch
     that is a multiple of 128, ``scale`` float32 ``[ceil(N / 128), ceil(K / 128)]``.  A value that is not finite becomes NaN."""
-    return _lib.host().quantize_weight(w)
+    if not torch.compiler.is_compiling():
+        out = _lib.host().quantize_weight(w)
+        if out is not None:
+            return out
+    return _weight_op(w.detach())
+
+
+@torch.library.custom_op("b200scan::quantize_weight", mutates_args=())
+def _weight_op(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return _lib.host().quant_weight(w)
+
+
+@_weight_op.register_fake
+def _(w):
+    (N, K), blocks = w.shape, lambda n: (n + 127) // 128
+    q = w.new_empty((N, 128 * blocks(K)), dtype=torch.uint8).view(torch.float8_e4m3fn).narrow(1, 0, K)
+    return q, w.new_empty((blocks(N), blocks(K)), dtype=torch.float32)
 
 
 @torch.library.custom_op("b200scan::quant_linear", mutates_args=())
 def _linear_op(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor:
-    return _lib.host().quant_linear(x, q, scale, bias)
+    return _lib.host().quant_product(x, q, scale, bias)
 
 
 @_linear_op.register_fake
@@ -43,4 +59,8 @@ def quant_linear(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, bias: to
     ``q`` and ``scale`` as ``quantize_weight`` returns them: the scales are powers of two, and another value gives NaN in the
     results that its block enters.  A ``q`` whose rows TMA cannot read (pitch or base not a multiple of 16 bytes) is copied first.  A row of x with a value that is not finite gives NaN
     throughout.  Sums are float32, the result is rounded once to x's type."""
-    return (_linear_op if torch.compiler.is_compiling() else _lib.host().quant_linear)(x, q, scale, bias)
+    if not torch.compiler.is_compiling():
+        out = _lib.host().quant_linear(x, q, scale, bias)
+        if out is not None:
+            return out
+    return _linear_op(x, q, scale, bias)
