@@ -134,3 +134,40 @@ def test_opcheck_of_the_weight():
 
     for shape in ((300, 200), (1, 128)):
         torch.library.opcheck(quant_b200._weight_op, (torch.randn(*shape, device="cuda"),), test_utils=("test_faketensor",))
+
+
+def test_second_derivatives_by_every_operand_are_refused():
+    """Gradients depend on the upstream gradients and on h0 too: asking for those derivatives raises as for the others, with
+    allow_unused as well, and so does the forward derivative that is made of two backward passes."""
+    import tsfast_b200 as b
+
+    x, r, i, lam, w = (t.requires_grad_() for t in tensors())
+    h0 = torch.randn(2, 24, device="cuda", requires_grad=True)
+    up, up_last = torch.randn(2, 37, 24, device="cuda", requires_grad=True), torch.randn(2, 24, device="cuda", requires_grad=True)
+    outs = b.gated_recurrence(x, r, i, lam, h0)
+    grads = torch.autograd.grad(outs, (x, r, i, lam, h0), (up, up_last), create_graph=True)
+    for g in grads:
+        for by in (up, up_last, h0, x, r, i, lam):
+            with pytest.raises(RuntimeError, match="no second derivative"):
+                torch.autograd.grad(g.sum(), by, retain_graph=True, allow_unused=True)
+    seam = b.residual_norm(x, i, w, gate=r)
+    for g in torch.autograd.grad(seam, (x, i, r, w), (up, up), create_graph=True):
+        for by in (up, x, i, r, w):
+            with pytest.raises(RuntimeError, match="no second derivative"):
+                torch.autograd.grad(g.sum(), by, retain_graph=True, allow_unused=True)
+    for f in (lambda t: b.gated_recurrence(t, r.detach(), i.detach(), lam.detach())[0], lambda t: b.gated_norm(t, r.detach(), w.detach())):
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            torch.autograd.functional.jvp(f, x.detach(), torch.ones_like(x))
+
+
+def test_the_start_may_be_overwritten_before_the_backward_pass():
+    """h0 is not kept for it: a cache may be used as h0 and go on."""
+    import tsfast_b200 as b
+
+    x, r, i, lam, _ = (t.requires_grad_() for t in tensors())
+    h0 = torch.randn(2, 24, device="cuda")
+    want = torch.autograd.grad(b.gated_recurrence(x, r, i, lam, h0)[0].sum(), (x, lam))
+    cache = h0.clone()
+    h, last = b.gated_recurrence(x, r, i, lam, cache)
+    cache.copy_(last.detach())
+    assert all(torch.equal(a, b_) for a, b_ in zip(torch.autograd.grad(h.sum(), (x, lam)), want))

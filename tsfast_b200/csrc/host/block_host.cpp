@@ -136,12 +136,16 @@ void check_sequences(const char* op, const Tensor& x, const Tensor& r, const Ten
     if (!(c > 0) || !std::isfinite(c)) refuse(op, "c=", c, ", a positive number is needed");
 }
 
-// Gradients that are not differentiable any further: their graph leads back to the operands through a node that raises.
-variable_list once(const char* op, variable_list grads, const variable_list& operands) {
+// Gradients that are not differentiable any further: their graph leads back through a node that raises to all that they depend on,
+// which are the running node's own operands (those that are not kept for it included) and the upstream gradients.
+variable_list once(const char* op, variable_list grads, const variable_list& upstream) {
     if (!at::GradMode::is_enabled()) return grads;
     torch::autograd::edge_list edges;
-    for (const auto& t : operands)
-        if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
+    if (const auto running = torch::autograd::get_current_node())
+        for (const auto& edge : running->next_edges())
+            if (edge.is_valid()) edges.push_back(edge);
+    for (const auto& g : upstream)
+        if (g.defined() && g.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(g));
     auto node = std::make_shared<torch::autograd::Error>(std::string("b200scan::") + op + ": there is no second derivative", std::move(edges));
     for (auto& g : grads)
         if (g.defined()) torch::autograd::create_gradient_edge(g, node);
@@ -219,7 +223,7 @@ struct GatedNode : Function<GatedNode> {
             at::NoGradGuard off;
             return gated_backward(g[0], g[1], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["c"].toDouble(), h0);
         }();
-        return once("gated_recurrence", {gx, gr, gi, glam, h0 ? gh0 : Tensor(), Tensor(), Tensor()}, s);
+        return once("gated_recurrence", {gx, gr, gi, glam, h0 ? gh0 : Tensor(), Tensor(), Tensor()}, g);
     }
 };
 
@@ -395,7 +399,7 @@ struct NormNode : Function<NormNode> {
                                   ctx->saved_data["act"].toInt(), ctx->saved_data["eps"].toDouble());
         }
         for (int k = 0; k < 3; ++k) grads.emplace_back();
-        return once("block_norm", grads, s);
+        return once("block_norm", grads, g);
     }
 };
 
