@@ -171,3 +171,27 @@ def test_the_start_may_be_overwritten_before_the_backward_pass():
     h, last = b.gated_recurrence(x, r, i, lam, cache)
     cache.copy_(last.detach())
     assert all(torch.equal(a, b_) for a, b_ in zip(torch.autograd.grad(h.sum(), (x, lam)), want))
+
+
+@pytest.mark.parametrize("name", [n for n in NAMES if n != "quantize_weight"])
+def test_forward_derivatives_are_refused(name):
+    """Not dropped: a dual tensor raises, and so does a tensor inside a transform of torch.func."""
+    import torch.autograd.forward_ad as fw
+
+    f, args = calls()[name], tensors()
+    with torch.no_grad():
+        with fw.dual_level():
+            for k in range(5):
+                dual = [fw.make_dual(t, torch.ones_like(t)) if j == k else t for j, t in enumerate(args)]
+                if any(a is not b for a, b in zip(dual, args)) and uses(name, k):
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        f(*dual)
+        if uses(name, 0):
+            with pytest.raises(RuntimeError, match="torch.func"):
+                torch.func.jvp(lambda x: f(x, *args[1:]), (args[0],), (torch.ones_like(args[0]),))
+            with pytest.raises(RuntimeError, match="torch.func"):
+                torch.vmap(lambda x: f(x, *args[1:]))(torch.stack([args[0], args[0]]))
+
+
+def uses(name, k):
+    return k in {"gated_norm": (0, 1, 4), "residual_norm": (0, 1, 2, 4), "quant_linear": (0,)}.get(name, (0, 1, 2, 3))

@@ -108,6 +108,16 @@ bool recorded(std::initializer_list<const Tensor*> operands) {
     return false;
 }
 
+// Derivatives and transforms that the operators do not have: without a refusal a dual tensor's tangent would be dropped
+void check_plain(const char* op, std::initializer_list<const Tensor*> operands) {
+    for (const Tensor* t : operands) {
+        if (!t->defined()) continue;
+        if (t->key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched})))
+            refuse(op, "it does not run inside the transforms of torch.func");
+        if (t->_fw_grad(0).defined()) refuse(op, "there is no forward-mode derivative");
+    }
+}
+
 Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::empty(sizes, like.options().dtype(type).memory_format(std::nullopt).requires_grad(false)); }
 Tensor workspace(size_t bytes, const Tensor& like) { return empty({(int64_t)std::max<size_t>(bytes, 256)}, at::kByte, like); }
 // unit stride along the last axis (a copy only if it is strided)
@@ -231,6 +241,7 @@ struct GatedNode : Function<GatedNode> {
 std::optional<std::tuple<Tensor, Tensor>> gated_recurrence(Tensor x, Tensor r, Tensor i, const Tensor& lam, Opt h0, const Opt& cu, double c) {
     const char* op = "gated_recurrence";
     const Tensor h0_ = get(h0), cu_ = get(cu);
+    check_plain(op, {&x, &r, &i, &lam, &h0_});
     if (recorded({&x, &r, &i, &lam, &h0_, &cu_})) return {};
     const bool shaped = !has(cu) && x.dim() != 3;
     std::vector<int64_t> lead;
@@ -298,6 +309,7 @@ std::optional<Tensor> gated_recurrence_step(const Tensor& x, const Tensor& r, co
     if (at::GradMode::is_enabled() && (x.requires_grad() || r.requires_grad() || i.requires_grad() || lam.requires_grad() || state.requires_grad()))
         refuse("gated_recurrence_step", "it has no gradient (call it under torch.no_grad(), or train with gated_recurrence)");
     const Tensor at = get(slots);
+    check_plain("gated_recurrence_step", {&x, &r, &i, &lam, &state});
     if (recorded({&x, &r, &i, &lam, &state, &at})) return {};
     return gated_step(x, r, i, lam, state, slots, c);
 }
@@ -408,6 +420,7 @@ std::optional<std::tuple<Tensor, Opt>> block_norm(const char* op, const Tensor& 
                                    const Opt& w2, const Opt& b2, int64_t kind, int64_t act, double eps) {
     const Params w = {get(w1), get(b1), get(scale), get(w2), get(b2)};
     const Tensor residual_ = get(residual), gate_ = get(gate);
+    check_plain(op, {&x, &residual_, &gate_, &w[0], &w[1], &w[2], &w[3], &w[4]});
     if (recorded({&x, &residual_, &gate_, &w[0], &w[1], &w[2], &w[3], &w[4]})) return {};
     check_norm(op, x, residual_, gate_, w, kind, eps);
     const bool flat = x.dim() == 2;
@@ -505,6 +518,7 @@ std::optional<Tensor> quant_linear(const Tensor& x, const Tensor& q, const Tenso
     if (at::GradMode::is_enabled() && (x.requires_grad() || scale.requires_grad() || wants(bias)))
         refuse("quant_linear", "it has no gradient (call it under torch.no_grad())");
     const Tensor b = get(bias);
+    check_plain("quant_linear", {&x, &q, &scale, &b});
     if (recorded({&x, &q, &scale, &b})) return {};
     return quant_product(x, q, scale, bias);
 }
