@@ -195,3 +195,19 @@ def test_forward_derivatives_are_refused(name):
 
 def uses(name, k):
     return k in {"gated_norm": (0, 1, 4), "residual_norm": (0, 1, 2, 4), "quant_linear": (0,)}.get(name, (0, 1, 2, 3))
+
+
+def test_constants_that_float32_does_not_hold_are_refused():
+    import tsfast_b200 as b
+
+    x, r, i, lam, w = tensors()
+    for c in (1e-60, 1e39, float("inf"), float("nan"), -1.0):
+        with pytest.raises(RuntimeError, match="c="):
+            b.gated_recurrence(x, r, i, lam, c=c)
+        with pytest.raises(RuntimeError, match="c="):
+            b.gated_recurrence_step(x[0], r[0], i[0], lam, torch.zeros(37, 24, device="cuda"), c=c)
+    for eps in (1e39, float("inf"), float("nan")):
+        with pytest.raises(RuntimeError, match="eps="):
+            b.gated_norm(x, r, w, eps=eps)
+        with pytest.raises(RuntimeError, match="eps="):
+            b.residual_norm(x, r, w, eps=eps)

@@ -143,7 +143,8 @@ void check_sequences(const char* op, const Tensor& x, const Tensor& r, const Ten
     check_like(op, "i", i, x);
     if (lam.scalar_type() != at::kFloat || lam.device() != x.device() || lam.dim() != 1 || lam.size(0) != x.size(-1))
         refuse(op, "lam is ", Say{lam}, ", expected float32 [", x.size(-1), "] on ", x.device());
-    if (!(c > 0) || !std::isfinite(c)) refuse(op, "c=", c, ", a positive number is needed");
+    const float c32 = (float)c;  // as the kernels take it
+    if (!(c32 > 0) || !std::isfinite(c32)) refuse(op, "c=", c, ", a positive number is needed, in the range of float32");
 }
 
 // Gradients that are not differentiable any further: their graph leads back through a node that raises to all that they depend on,
@@ -342,7 +343,7 @@ void check_norm(const char* op, const Tensor& x, const Tensor& residual, const T
         first = &t;
     }
     if (kind == 0 && (w[1].defined() || w[4].defined())) refuse(op, "a bias goes with kind=\"layer\", an RMS norm has none");
-    if (!(eps >= 0) || !std::isfinite(eps)) refuse(op, "eps=", eps, ", a number that is not negative is needed");
+    if (!(eps >= 0) || !std::isfinite((float)eps)) refuse(op, "eps=", eps, ", a number that is not negative is needed, in the range of float32");
 }
 
 // rows [M, D]; returns y, residual' (undefined without a residual) and the statistics (undefined unless `keep`)
