@@ -211,3 +211,18 @@ def test_constants_that_float32_does_not_hold_are_refused():
             b.gated_norm(x, r, w, eps=eps)
         with pytest.raises(RuntimeError, match="eps="):
             b.residual_norm(x, r, w, eps=eps)
+
+
+def test_a_cache_of_inference_mode():
+    """It may be updated inside that mode only, as for every operator that updates a tensor; a refused call leaves it as it was."""
+    import tsfast_b200 as b
+
+    x, r, i, lam, _ = tensors()
+    with torch.inference_mode():
+        state = torch.zeros(37, 24, device="cuda")
+        b.gated_recurrence_step(x[0], r[0], i[0], lam, state)
+        kept = state.clone()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="nference"):
+        b.gated_recurrence_step(x[0], r[0], i[0], lam, state)
+    with torch.inference_mode():
+        assert torch.equal(state, kept) and state.abs().sum() > 0

@@ -297,13 +297,13 @@ Tensor gated_step(const Tensor& x_, const Tensor& r_, const Tensor& i_, const Te
         refuse(op, B, " rows and ", n, " states: without slots row b has state b");
     }
     const Tensor x = unit(x_), r = unit(r_), i = unit(i_), lam = dense(lam_);
+    state.unsafeGetTensorImpl()->bump_version();  // raises for a tensor of inference mode outside of it: before the update
     Launch on(x);
     Tensor h = empty({B, D}, x.scalar_type(), x);
     check(lib.b200_gated_step(tag_of(x.scalar_type()), B, D, n, (float)c, x.data_ptr(), x.stride(0), r.data_ptr(), r.stride(0), i.data_ptr(), i.stride(0),
                               lam.data_ptr(), state.data_ptr(), std::max(state.stride(0), D), ptr(slots), slots.defined() && slots.scalar_type() == at::kLong,
                               h.data_ptr(), on.stream()),
           "b200_gated_step");
-    state.unsafeGetTensorImpl()->bump_version();
     return h;
 }
 std::optional<Tensor> gated_recurrence_step(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam, const Tensor& state, const Opt& slots, double c) {
