@@ -226,3 +226,27 @@ def test_a_cache_of_inference_mode():
         b.gated_recurrence_step(x[0], r[0], i[0], lam, state)
     with torch.inference_mode():
         assert torch.equal(state, kept) and state.abs().sum() > 0
+
+
+def test_compiled_calls_refuse_what_eager_ones_refuse():
+    """A norm without its weight would return memory that nothing wrote."""
+    import tsfast_b200 as b
+
+    x, r, i, lam, w = tensors()
+    compiled = lambda f: torch.compile(f, backend="aot_eager")  # noqa: E731
+    with torch.no_grad():
+        with pytest.raises(Exception, match="weight is required"):
+            compiled(lambda x, r, w: b.residual_norm(x, r, None, post_weight=w))(x, r, w)
+        with pytest.raises(Exception, match="weight is required"):
+            compiled(lambda x, r: b.gated_norm(x, r, None))(x, r)
+        with pytest.raises(Exception, match="post_bias without post_weight"):
+            compiled(lambda x, r, w: b.residual_norm(x, r, w, post_bias=w, kind="layer"))(x, r, w)
+        with pytest.raises(Exception, match="residual is required"):
+            compiled(lambda x, w: b.residual_norm(x, None, w))(x, w)
+        wide = x.reshape(2, 1, 37, 24)
+        with pytest.raises(Exception, match="r is"):
+            compiled(lambda x, r, lam: b.gated_recurrence(x, r, x, lam))(wide, wide.transpose(0, 1).contiguous(), lam)
+        with pytest.raises(Exception, match="h0 is"):
+            compiled(lambda x, lam, h: b.gated_recurrence(x, x, x, lam, h))(wide, lam, torch.zeros(1, 2, 24, device="cuda"))
+        h, last = compiled(lambda x, lam: b.gated_recurrence(x, x, x, lam))(wide[:, :, :0], lam)
+        assert h.shape == (2, 1, 0, 24) and (last == 0).all()

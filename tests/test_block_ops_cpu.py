@@ -106,3 +106,18 @@ def test_packed_tiles_never_share_a_slot(built):
             cu = sorted(rng.choices(range(T + 1), k=rng.randrange(1, 9)))
             used = [cu[s] // tile + s + k for s in range(len(cu) - 1) for k in range(-(-(cu[s + 1] - cu[s]) // tile))]
             assert len(set(used)) == len(used) and all(u < built.lib().b200_gated_chk_rows(tag, len(cu) - 1, 0, T, 1) for u in used)
+
+
+def test_norms_without_their_weight_are_refused_on_every_way(built):
+    """The custom op checks like the eager call: without a weight it would leave its result unwritten."""
+    from tsfast_b200 import norm_b200
+
+    x, w = torch.zeros(3, 8), torch.ones(8)
+    with pytest.raises(RuntimeError, match="weight is required"):
+        norm_b200._norm_op(x, x, None, w, None, None, None, None, 0, 1, 1e-6)
+    with pytest.raises(RuntimeError, match="weight is required"):
+        norm_b200._norm_op(x, None, x, None, None, None, None, None, 0, 1, 1e-6)
+    with pytest.raises(RuntimeError, match="post_bias without post_weight"):
+        norm_b200._norm_op(x, x, None, None, w, None, w, None, 1, 1, 1e-6)
+    with pytest.raises(RuntimeError, match="residual is required"):
+        norm_b200._norm_op(x, None, None, None, None, None, w, None, 0, 1, 1e-6)

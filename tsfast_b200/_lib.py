@@ -147,6 +147,12 @@ def host():
     return _HOST
 
 
+def check_shape(op: str, name: str, t, expected, like: str = "") -> None:
+    """Refuse an operand of another shape where the call is about to reshape it (the host path checks for itself)."""
+    if t is not None and t.shape != expected:
+        raise RuntimeError(f"b200scan::{op}: {name} is {list(t.shape)}, expected {list(expected)}{like}")
+
+
 def workspace(nbytes: int, device) -> torch.Tensor:
     """Scratch for one call, from torch's caching allocator (legal under graph capture)."""
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)

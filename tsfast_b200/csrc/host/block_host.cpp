@@ -326,6 +326,9 @@ int params_f32(const Params& w) { return (w[3].defined() ? w[3] : w[0]).scalar_t
 
 // without a residual the parameters are those of the gated norm, which calls its own "weight" and "bias"
 void check_norm(const char* op, const Tensor& x, const Tensor& residual, const Tensor& gate, const Params& w, int64_t kind, double eps) {
+    if (!residual.defined() && (w[2].defined() || w[3].defined())) refuse(op, "residual is required");
+    if (!(residual.defined() ? w[3] : w[0]).defined()) refuse(op, "weight is required");
+    if (w[1].defined() && !w[0].defined()) refuse(op, "post_bias without post_weight: the norm of x is given by its weight");
     check_cuda_type(op, x);
     const int64_t D = x.dim() ? x.size(-1) : 0;
     if (D < 1 || D > kNormWidth) refuse(op, "rows of ", D, " features, the kernel takes 1 to ", kNormWidth);
@@ -444,15 +447,12 @@ std::optional<std::tuple<Tensor, Opt>> block_norm(const char* op, const Tensor& 
 }
 
 std::optional<Tensor> gated_norm(const Tensor& x, const Opt& gate, const Opt& weight, const Opt& bias, int64_t kind, int64_t act, double eps) {
-    if (!has(weight)) refuse("gated_norm", "weight is required");
     const auto out = block_norm("gated_norm", x, {}, gate, weight, bias, {}, {}, {}, kind, act, eps);
     return out ? std::optional(std::get<0>(*out)) : std::nullopt;
 }
-std::optional<std::tuple<Tensor, Opt>> residual_norm(const Tensor& x, const Opt& residual, const Opt& weight, const Opt& bias, const Opt& gate, const Opt& scale,
-                                      const Opt& post_weight, const Opt& post_bias, int64_t kind, int64_t act, double eps) {
-    if (!has(residual)) refuse("residual_norm", "residual is required");
-    if (!has(weight)) refuse("residual_norm", "weight is required");
-    if (has(post_bias) && !has(post_weight)) refuse("residual_norm", "post_bias without post_weight: the norm of x is given by its weight");
+std::optional<std::tuple<Tensor, Opt>> residual_norm(const Tensor& x, const Opt& residual, const Opt& weight, const Opt& bias, const Opt& gate,
+                                                     const Opt& scale, const Opt& post_weight, const Opt& post_bias, int64_t kind, int64_t act, double eps) {
+    if (!has(residual)) refuse("residual_norm", "residual is required");  // (else it might pass for a gated norm)
     return block_norm("residual_norm", x, residual, gate, post_weight, post_bias, scale, weight, bias, kind, act, eps);
 }
 

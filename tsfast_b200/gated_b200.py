@@ -98,8 +98,13 @@ def gated_recurrence(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, lam: tor
             return out
     if cu_seqlens is not None or x.dim() == 3:
         return _gated_op(x, r, i, lam, h0, cu_seqlens, float(c))[:2]
+    if x.dim() < 2:
+        raise RuntimeError(f"b200scan::gated_recurrence: x is {list(x.shape)}, expected at least [L, D]")
     lead, tail = x.shape[:-2], x.shape[-2:]
     n = math.prod(lead)
+    for name, t in (("r", r), ("i", i)):
+        _lib.check_shape("gated_recurrence", name, t, x.shape, " like x")
+    _lib.check_shape("gated_recurrence", "h0", h0, (*lead, tail[1]))
     h, last, _ = _gated_op(*(t.reshape(n, *tail) for t in (x, r, i)), lam, None if h0 is None else h0.reshape(n, tail[1]), None, float(c))
     return h.reshape(x.shape), last.reshape(*lead, tail[1])
 

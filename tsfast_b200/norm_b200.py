@@ -96,7 +96,9 @@ def _codes(op, kind, activation):
                            "'sigmoid' or None") from None
 
 
-def _composed(x, residual, gate, params, kind, act, eps):
+def _composed(op, x, residual, gate, params, kind, act, eps):
+    for name, t in (("residual", residual), ("gate", gate)):
+        _lib.check_shape(op, name, t, x.shape, " like x")
     flat = lambda t: None if t is None else t.reshape(-1, x.shape[-1])  # noqa: E731
     y, r, _ = _norm_op(flat(x), flat(residual), flat(gate), *params, kind, act, float(eps))
     return y.reshape(x.shape), r if residual is None else r.reshape(x.shape)
@@ -111,7 +113,7 @@ def gated_norm(x: torch.Tensor, gate: torch.Tensor | None, weight: torch.Tensor,
         out = _lib.host().gated_norm(x, gate, weight, bias, kind, act, eps)
         if out is not None:
             return out
-    return _composed(x, None, gate, (weight, bias, None, None, None), kind, act, eps)[0]
+    return _composed("gated_norm", x, None, gate, (weight, bias, None, None, None), kind, act, eps)[0]
 
 
 def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -128,4 +130,6 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
         out = _lib.host().residual_norm(x, residual, weight, bias, gate, scale, post_weight, post_bias, kind, act, eps)
         if out is not None:
             return out
-    return _composed(x, residual, gate, (post_weight, post_bias, scale, weight, bias), kind, act, eps)
+    if residual is None:  # (else it might pass for a gated norm)
+        raise RuntimeError("b200scan::residual_norm: residual is required")
+    return _composed("residual_norm", x, residual, gate, (post_weight, post_bias, scale, weight, bias), kind, act, eps)
