@@ -478,14 +478,14 @@ quant_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         const int quarter = wid & 3, half = (wid - 4) >> 2;
         const uint32_t column0 = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * HC);
         long long ti = 0;
-        for (long long t = t0; t < tiles && !abort_flag; t += dt, ++ti) {
+        for (long long t = t0; t < tiles; t += dt, ++ti) {
             const int n = (int)(t % n_tiles) * kWide + member * kFeatures + quarter * 32 + lane;
             const long long m0 = t / n_tiles * TN + half * HC;
             const float bias = p.bias == nullptr || n >= p.N || p.split > 1 ? 0.f
                                : p.bias_f32                                ? static_cast<const float*>(p.bias)[n]
                                                                            : to_float(static_cast<const T*>(p.bias)[n]);
-            if (!wait(&acc_full, (uint32_t)(ti & 1))) break;
-            __syncwarp();
+            // the warp leaves as one: the loads from tensor memory want all of its lanes, and lanes may see the flag at different polls
+            if (!__all_sync(0xffffffffu, wait(&acc_full, (uint32_t)(ti & 1)))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float* part = reinterpret_cast<float*>(base);  // (clusters) where the operands' blocks were: all of them have been read
             T out[HC];
