@@ -383,6 +383,12 @@ size_t b200_quant_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int b200_quant_linear(int dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* q, int64_t ldq,
                       const void* scale, const void* bias, int bias_f32, void* y, int64_t ldy, void* workspace,
                       size_t workspace_bytes, void* stream);
+/* Test probe: the same call with the polls that a wait makes before it gives up (0 = the default, about a second) and
+ * a tile (features first, then tokens; -1 = none) whose end is not reported, so that the waits for it run out, the launch
+ * returns and b200_block_status reports B200_ERR_TIMEOUT. */
+int b200_quant_probe(int polls, int64_t mute_tile, int dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
+                     const void* q, int64_t ldq, const void* scale, const void* bias, int bias_f32, void* y, int64_t ldy,
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -79,6 +79,7 @@ SIGNATURES = {
     "b200_quant_weight": (_int, [_int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
     "b200_quant_linear_workspace_bytes": (_sz, [_i64] * 3),
     "b200_quant_linear": (_int, [_int, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _int, _vp, _i64, _vp, _sz, _vp]),
+    "b200_quant_probe": (_int, [_int, _i64, _int, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _int, _vp, _i64, _vp, _sz, _vp]),
     "b200_gated_step": (_int, [_int] + [_i64] * 3 + [_f32] + [_vp, _i64] * 3 + [_vp, _vp, _i64, _vp, _int, _vp, _vp]),
 }
 

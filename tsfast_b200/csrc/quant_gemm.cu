@@ -42,7 +42,7 @@ constexpr int kFeatures = 128;   // rows of the first operand
 constexpr int kThreads = 384;
 constexpr int kStorers = 256;    // threads of warps 4-11
 constexpr int kMaxSplit = 8;
-constexpr int kWaitLimit = 1 << 18;  // polls of an mbarrier (each waits a while itself) before a wait gives up
+constexpr int kWaitLimit = 1 << 18;  // polls of an mbarrier before a wait gives up: about a second, a poll waits 4 us itself
 
 template <int TN, bool PAIR>
 struct Shape {
@@ -203,6 +203,8 @@ struct Args {
     const void* bias;
     int bias_f32;
     int split;        // CTAs of a cluster, each with its part of K
+    int polls;        // of a wait
+    long long mute;   // a tile whose end is not reported (-1: none)
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -363,7 +365,7 @@ quant_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
         const uint32_t a = smem_u32(bar);
-        for (int i = 0; i < kWaitLimit; ++i) {
+        for (int i = 0; i < p.polls; ++i) {
             uint32_t ok;
             if constexpr (PAIR)
                 asm volatile(
@@ -471,7 +473,7 @@ quant_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
                     if (++s == S::stages) s = 0, phase ^= 1u;
                 }
                 if (!fine) break;
-                umma_commit<PAIR>(&acc_full);
+                if (t != p.mute) umma_commit<PAIR>(&acc_full);
             }
         }
     } else if (wid >= 4) {
@@ -548,12 +550,15 @@ quant_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         }
         cluster_sync();  // nobody leaves while its part is being read
     }
-    if (abort_flag && tid == 0) {
-        atomicExch(&product_lost, (unsigned int)B200_ERR_TIMEOUT);
-        for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies in flight get a bounded time to land
-    }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (abort_flag) {  // (whoever gave up, all of the block are here, and see it)
+        if (tid == 0) {
+            atomicExch(&product_lost, (unsigned int)B200_ERR_TIMEOUT);
+            for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies in flight get a bounded time to land
+        }
+        __syncthreads();
+    }
     if constexpr (PAIR) {
         cluster_sync();  // neither leaves while the other's barriers or blocks are in use
         if (wid == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::cols) : "memory");
@@ -692,8 +697,8 @@ size_t b200_quant_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     return b200::quant::plan(M, N, K).total;
 }
 
-int b200_quant_linear(int dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* q, int64_t ldq, const void* scale,
-                      const void* bias, int bias_f32, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
+int b200_quant_probe(int polls, int64_t mute_tile, int dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* q, int64_t ldq,
+                     const void* scale, const void* bias, int bias_f32, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace b200;
     using namespace b200::quant;
     if ((dtype != B200_BF16 && dtype != B200_F16) || M < 0 || N < 1 || K < 1 || N > (1 << 22) || K > (1 << 22) || M > 0x7fffff00LL) return B200_ERR_ARG;
@@ -703,9 +708,15 @@ int b200_quant_linear(int dtype, int64_t M, int64_t N, int64_t K, const void* x,
     if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < w.total) return B200_ERR_WORKSPACE;
     Args p = {};
     p.y = y, p.ldy = ldy, p.M = M, p.N = (int)N, p.bias = bias, p.bias_f32 = bias_f32;
+    p.polls = polls > 0 && polls < kWaitLimit ? polls : kWaitLimit, p.mute = mute_tile;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return dtype == B200_BF16 ? run<__nv_bfloat16>(x, ldx, q, ldq, (const float*)scale, (int)K, w, (char*)workspace, p, st)
                               : run<__half>(x, ldx, q, ldq, (const float*)scale, (int)K, w, (char*)workspace, p, st);
+}
+
+int b200_quant_linear(int dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* q, int64_t ldq, const void* scale,
+                      const void* bias, int bias_f32, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
+    return b200_quant_probe(0, -1, dtype, M, N, K, x, ldx, q, ldq, scale, bias, bias_f32, y, ldy, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"
