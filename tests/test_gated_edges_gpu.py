@@ -154,3 +154,38 @@ def test_channels_that_hardly_change():
     beta2 = -torch.expm1(2 * want["l"])
     near(got[2], want["gx"].expand_as(got[2]), 72 * U + TINY / beta2 / 2, "gx")
     near(got[0], want["h"].expand_as(got[0]), 72 * U, "h")
+
+
+# one CTA per chain, clusters of several, packed sequences, either width of a lane
+@pytest.mark.parametrize("dt,S,L,D,mute", [(torch.float32, 2, 100, 30, 0), (torch.bfloat16, 300, 60, 256, 1), (torch.float32, 1, 3000, 64, 3),
+                                           (torch.bfloat16, 8, 2000, 1024, 2), (torch.bfloat16, 1, 2000, 40, 0)])
+def test_a_wait_that_runs_out_is_reported(dt, S, L, D, mute):
+    """A step whose result is kept back (the probe's mute step): the waits for it give up, the launch ends and the error word says so,
+    once; what came before is right, and so is the next call."""
+    import tsfast_b200 as b
+    from tsfast_b200 import _lib
+
+    lib = _lib.lib()
+    g = torch.Generator(device="cuda").manual_seed(L)
+    x, r, i = (torch.randn(S, L, D, device="cuda", generator=g).to(dt) for _ in range(3))
+    lam = torch.randn(D, device="cuda", generator=g) - 5
+    stream = _lib.stream_ptr(x.device)
+    with torch.no_grad():
+        want, last = b.gated_recurrence(x, r, i, lam)
+    assert lib.b200_block_status(stream) == 0
+    tag = {torch.float32: 0, torch.bfloat16: 2}[dt]
+
+    def probe(mute, polls):
+        h, end = torch.zeros_like(want), torch.zeros_like(last)
+        assert lib.b200_gated_probe(polls, mute, tag, S, L, 0, D, 8.0, None, 0, *(a for t in (x, r, i) for a in (_lib.ptr(t), L * D, D)), _lib.ptr(lam),
+                                    None, _lib.ptr(h), _lib.ptr(end), None, stream) == 0
+        return h, end
+
+    assert all(torch.equal(a, w) for a, w in zip(probe(-1, 0), (want, last))) and lib.b200_block_status(stream) == 0
+    h, _ = probe(mute, 64)
+    assert lib.b200_block_status(stream) == 5  # B200_ERR_TIMEOUT
+    assert lib.b200_block_status(stream) == 0
+    assert torch.equal(h[:, : 28 * mute], want[:, : 28 * mute])  # (later values are whatever shared memory held: the last call's, even)
+    with torch.no_grad():
+        again, last_again = b.gated_recurrence(x, r, i, lam)
+    assert torch.equal(again, want) and torch.equal(last_again, last) and lib.b200_block_status(stream) == 0

@@ -218,6 +218,7 @@ struct Args {
     int ctiles, C;
     float c;
     int whole;          // outputs: rows of whole lanes of channels on an aligned base
+    int polls, mute;    // forward: polls of a wait; a step whose result the first CTA of every chain keeps to itself (-1: none)
 };
 
 __device__ __forceinline__ long long boundary(const Args& p, long long k) {
@@ -352,10 +353,11 @@ __device__ __forceinline__ void expect(uint64_t* bar, int bytes) {
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// Bounded wait. One that runs out is remembered in `lost`: later waits return at once, the results are wrong, and the
-// error word says so.
-__device__ __forceinline__ void await(uint64_t* bar, uint32_t parity, bool& lost) {
-    for (int i = 0; i < kSpinLimit && !lost; ++i) {
+// Bounded wait (a poll waits 4 us itself). One that runs out is remembered in `lost`: later waits return at once, the results are
+// wrong, and the error word says so.
+constexpr int kWaitLimit = 1 << 18;  // polls: about a second
+__device__ __forceinline__ void await(uint64_t* bar, uint32_t parity, int polls, bool& lost) {
+    for (int i = 0; i < polls && !lost; ++i) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -371,7 +373,7 @@ __device__ __forceinline__ void await(uint64_t* bar, uint32_t parity, bool& lost
 
 // What the warps of a CTA, and the CTAs of a cluster, tell one another; two of each, for alternating tiles.
 struct Barriers {
-    uint64_t maps[2];   // the eight warps' maps are written
+    uint64_t maps[2];   // the seven warps' maps are written
     uint64_t start[2];  // the states that enter the segments are written
     uint64_t peers[2];  // the tiles' maps of all CTAs have come in
 };
@@ -390,20 +392,30 @@ __device__ __forceinline__ void open_exchange(int C, Barriers& b) {
 __device__ unsigned int exchange_lost;  // B200_ERR_TIMEOUT once a wait ran out
 __device__ __forceinline__ void close_exchange(int C, bool lost) {
     if (lost) atomicExch(&exchange_lost, (unsigned int)B200_ERR_TIMEOUT);
-    if (C > 1) cluster_sync();  // nobody leaves while a map may be on its way to it
-    else __syncthreads();
+    if (C > 1) {
+        cluster_sync();  // nobody leaves while a map may be on its way to it: all have been sent, and who has not lost a wait has them all
+        if (__syncthreads_or(lost))
+            for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // who has lost one gives the rest a bounded time to land
+    } else {
+        __syncthreads();
+    }
 }
 // The folding warp of every CTA tells all CTAs of its cluster its tile's maps, and folds theirs from the carry: the states
 // that enter this CTA's tile (in `enter`); the carry becomes those behind the last CTA's.
+// A lane that has lost a wait sends and expects nothing any more (the barrier would be arrived at twice in one phase), so all
+// CTAs lose theirs.
 template <int NP>
 __device__ __forceinline__ void exchange(Map (*peers)[NP][32], Barriers& b, int C, int rank, int s, const Map (&mine)[NP], Pair (&enter)[NP],
-                                         Pair (&carry)[NP], bool& lost) {
+                                         Pair (&carry)[NP], int polls, int mute, bool& lost) {
     const int buf = s & 1, lane = threadIdx.x & 31;
-    if (lane == 0) expect(&b.peers[buf], C * 32 * NP * (int)sizeof(Map));
-    for (int c = 0; c < C; ++c)
+    if (!lost) {
+        if (lane == 0) expect(&b.peers[buf], C * 32 * NP * (int)sizeof(Map));
+        if (s != mute || rank != 0)
+            for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int k = 0; k < NP; ++k) put_remote(&peers[buf * C + rank][k][lane], &b.peers[buf], c, mine[k]);
-    await(&b.peers[buf], (uint32_t)(s >> 1) & 1u, lost);
+                for (int k = 0; k < NP; ++k) put_remote(&peers[buf * C + rank][k][lane], &b.peers[buf], c, mine[k]);
+        await(&b.peers[buf], (uint32_t)(s >> 1) & 1u, polls, lost);
+    }
     for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
@@ -459,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const Args p) {
         if (p.h0 != nullptr) load_state<NP>(p.h0 + seq * p.D + d, n, carry);
         for (int s = 0; s < steps; ++s) {
             const int buf = s & 1, tile = s * C + rank;
-            await(&bars.maps[buf], (uint32_t)(s >> 1) & 1u, lost);
+            await(&bars.maps[buf], (uint32_t)(s >> 1) & 1u, p.polls, lost);
             if (C == 1) {
 #pragma unroll
                 for (int k = 0; k < NP; ++k) h[k] = carry[k];
@@ -471,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const Args p) {
 #pragma unroll
                     for (int w = 1; w < kWarps; ++w) whole[k] = after(maps[buf][w][k][lane], whole[k]);
                 }
-                exchange<NP>(peers, bars, C, rank, s, whole, h, carry, lost);
+                exchange<NP>(peers, bars, C, rank, s, whole, h, carry, p.polls, p.mute, lost);
             }
             if (p.chk != nullptr && tile < tiles) store_state<NP>(p.chk + (ch.slot0 + tile) * p.D + d, n, h);
 #pragma unroll
@@ -486,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const Args p) {
                 for (int k = 0; k < NP; ++k) carry[k] = h[k];
             }
             __syncwarp();
-            if (lane == 0) arrive(&bars.start[buf]);
+            if (lane == 0 && (C > 1 || s != p.mute)) arrive(&bars.start[buf]);
         }
         if (rank == 0) store_state<NP>(p.hlast + seq * p.D + d, n, carry);
     } else {
@@ -557,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const Args p) {
         auto states = [&](int s, const Pair(&a)[TS][NP], const Pair(&b)[TS][NP]) {
             const int row0 = (s * C + rank) * kTile + wid * TS, left = ch.len - row0;
             T* out = static_cast<T*>(p.out[0]) + (ch.row0 + row0) * p.D + d;
-            await(&bars.start[s & 1], (uint32_t)(s >> 1) & 1u, lost);
+            await(&bars.start[s & 1], (uint32_t)(s >> 1) & 1u, p.polls, lost);
             Pair h[NP];
 #pragma unroll
             for (int e = 0; e < NP; ++e) h[e] = start[s & 1][wid][e][lane];
@@ -631,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
 #pragma unroll
             for (int k = 0; k < NP; ++k) h[k] = next[k];
             kept(s + 1);
-            await(&bars.maps[buf], (uint32_t)(s >> 1) & 1u, lost);
+            await(&bars.maps[buf], (uint32_t)(s >> 1) & 1u, kWaitLimit, lost);
             if (C == 1) {
 #pragma unroll
                 for (int k = 0; k < NP; ++k) g[k] = carry[k];
@@ -643,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
 #pragma unroll
                     for (int w = kWarps - 2; w >= 0; --w) whole[k] = after(maps[buf][w][k][lane], whole[k]);
                 }
-                exchange<NP>(peers, bars, C, rank, s, whole, g, carry, lost);
+                exchange<NP>(peers, bars, C, rank, s, whole, g, carry, kWaitLimit, -1, lost);
             }
 #pragma unroll
             for (int k = 0; k < NP; ++k) {
@@ -751,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
         };
         auto gradients = [&](int s, const Coeffs& f) {
             const int row0 = first_row(s), left = row0 < 0 ? 0 : ch.len - row0;
-            await(&bars.start[s & 1], (uint32_t)(s >> 1) & 1u, lost);
+            await(&bars.start[s & 1], (uint32_t)(s >> 1) & 1u, kWaitLimit, lost);
             Pair g[NP], before[TS][NP], x[NP];
 #pragma unroll
             for (int e = 0; e < NP; ++e) {
@@ -1072,6 +1084,12 @@ int64_t b200_gated_chk_rows(int dtype, int64_t S, int64_t L, int64_t T, int pack
 int b200_gated_fwd(int dtype, int64_t S, int64_t L, int64_t T, int64_t D, float c, const void* cu, int cu_is64, const void* x, int64_t xb,
                    int64_t xt, const void* r, int64_t rb, int64_t rt, const void* i, int64_t ib, int64_t it, const void* lam, const void* h0,
                    void* h, void* hlast, void* chk, void* stream) {
+    return b200_gated_probe(0, -1, dtype, S, L, T, D, c, cu, cu_is64, x, xb, xt, r, rb, rt, i, ib, it, lam, h0, h, hlast, chk, stream);
+}
+
+int b200_gated_probe(int polls, int mute_step, int dtype, int64_t S, int64_t L, int64_t T, int64_t D, float c, const void* cu, int cu_is64, const void* x,
+                     int64_t xb, int64_t xt, const void* r, int64_t rb, int64_t rt, const void* i, int64_t ib, int64_t it, const void* lam,
+                     const void* h0, void* h, void* hlast, void* chk, void* stream) {
     using namespace b200;
     using namespace b200::gated;
     if (!sizes_ok(dtype, S, L, T, D)) return B200_ERR_ARG;
@@ -1083,6 +1101,7 @@ int b200_gated_fwd(int dtype, int64_t S, int64_t L, int64_t T, int64_t D, float 
     p.in[0] = {x, xb, xt}, p.in[1] = {r, rb, rt}, p.in[2] = {i, ib, it};
     p.out[0] = h, p.lam = (const float*)lam, p.h0 = (const float*)h0, p.hlast = (float*)hlast, p.chk = (float*)chk;
     p.cu = cu, p.cu64 = cu_is64, p.S = S, p.L = L, p.T = T, p.D = (int)D, p.c = c;
+    p.polls = polls > 0 && polls < kWaitLimit ? polls : kWaitLimit, p.mute = mute_step;
     return dispatch(dtype, false, p, S, rows, static_cast<cudaStream_t>(stream));
 }
 
