@@ -121,3 +121,66 @@ def test_norms_without_their_weight_are_refused_on_every_way(built):
         norm_b200._norm_op(x, x, None, None, w, None, w, None, 1, 1, 1e-6)
     with pytest.raises(RuntimeError, match="residual is required"):
         norm_b200._norm_op(x, None, None, None, None, None, w, None, 0, 1, 1e-6)
+
+
+def test_c_entry_points_refuse_pointers_off_their_elements(built):
+    """A pointer that is not on its element's boundary (or on 16 bytes, for the statistics) would fault on the device."""
+    L = built.lib()
+    z, base = ctypes.c_void_p(None), 1 << 20  # never dereferenced
+    at = lambda off=0: ctypes.c_void_p(base + off)  # noqa: E731
+
+    def norm_fwd(dtype=2, pf32=1, **off):
+        o = lambda n: at(off.get(n, 0))  # noqa: E731
+        return L.b200_block_norm_fwd(dtype, 3, 8, 1, 1, 1e-6, pf32, o("x"), 8, o("gate"), 8, o("residual"), 8, o("w1"), o("b1"), o("scale"), o("w2"),
+                                     o("b2"), o("y"), o("residual_out"), o("stats"), z)
+
+    def norm_bwd(dtype=2, pf32=1, **off):
+        o = lambda n: at(off.get(n, 0))  # noqa: E731
+        return L.b200_block_norm_bwd(dtype, 3, 8, 1, 1, 1e-6, pf32, o("gy"), 8, o("gres"), 8, o("x"), 8, o("gate"), 8, o("residual"), 8, o("w1"), o("b1"),
+                                     o("scale"), o("w2"), o("b2"), o("stats"), o("gx"), o("ggate"), o("gresidual"), o("gw1"), o("gb1"), o("gscale"),
+                                     o("gw2"), o("gb2"), at(), 1 << 30, z)
+
+    rows, params = ("x", "gate", "residual"), ("w1", "b1", "scale", "w2", "b2")
+    for name in (*rows, "y", "residual_out"):
+        assert norm_fwd(**{name: 1}) == 1 and norm_fwd(dtype=0, **{name: 2}) == 1, name
+    for name in (*rows, "gy", "gres", "gx", "ggate", "gresidual"):
+        assert norm_bwd(**{name: 1}) == 1 and norm_bwd(dtype=0, **{name: 2}) == 1, name
+    for name in params:
+        assert norm_fwd(**{name: 2}) == 1 and norm_fwd(pf32=0, **{name: 1}) == 1 and norm_bwd(**{name: 2}) == 1, name
+    for name in ("gw1", "gb1", "gscale", "gw2", "gb2"):
+        assert norm_bwd(**{name: 2}) == 1 and norm_bwd(pf32=0, **{name: 1}) == 1, name
+    for off in (4, 8):
+        assert norm_fwd(stats=off) == 1 and norm_bwd(stats=off) == 1
+
+    seq = (at(), 8, 8)
+
+    def fwd(cu=z, cu64=0, **off):
+        o = lambda n: at(off.get(n, 0))  # noqa: E731
+        return L.b200_gated_fwd(2, 1, 4, 4, 8, 8.0, cu, cu64, *seq, *seq, *seq, o("lam"), o("h0"), o("h"), o("last"), o("chk"), z)
+
+    for name in ("lam", "h0", "last", "chk"):
+        assert fwd(**{name: 2}) == 1, name
+    assert fwd(h=1) == 1 and fwd(cu=at(2)) == 1 and fwd(cu=at(4), cu64=1) == 1
+
+    def bwd(cu=z, cu64=0, **off):
+        o = lambda n: at(off.get(n, 0))  # noqa: E731
+        return L.b200_gated_bwd(2, 1, 4, 4, 8, 8.0, cu, cu64, *seq, *seq, *seq, o("lam"), o("chk"), *seq, o("glast"), o("gx"), o("gr"), o("gi"), o("glam"),
+                                o("gh0"), at(), 1 << 30, z)
+
+    for name in ("lam", "chk", "glast", "glam", "gh0"):
+        assert bwd(**{name: 2}) == 1, name
+    assert bwd(gr=1) == 1 and bwd(cu=at(2)) == 1 and bwd(cu=at(4), cu64=1) == 1
+
+    def step(slots64=0, **off):
+        o = lambda n: at(off.get(n, 0))  # noqa: E731
+        return L.b200_gated_step(2, 1, 8, 4, 8.0, o("x"), 8, o("r"), 8, o("i"), 8, o("lam"), o("state"), 8, o("slots"), slots64, o("h"), z)
+
+    assert step(x=1) == step(h=1) == step(lam=2) == step(state=2) == step(slots=2) == step(slots64=1, slots=4) == 1
+
+    def lin(bias_f32=1, **off):
+        o = lambda n: at(off.get(n, 0))  # noqa: E731
+        return L.b200_quant_linear(2, 4, 16, 32, o("x"), 32, o("q"), 32, o("scale"), o("bias"), bias_f32, o("y"), 16, at(), 1 << 30, z)
+
+    assert lin(x=1) == lin(y=1) == lin(scale=2) == lin(bias=2) == lin(bias_f32=0, bias=1) == 1
+    weight = lambda dtype=0, w=0, scale=0: L.b200_quant_weight(dtype, 4, 4, at(w), 4, at(), 4, at(scale), z)  # noqa: E731
+    assert weight(w=2) == weight(dtype=2, w=1) == weight(scale=2) == 1

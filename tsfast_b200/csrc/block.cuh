@@ -89,6 +89,11 @@ inline int take_error_word(unsigned int& word, cudaStream_t st) {
     return (int)error;
 }
 
+// whether every pointer is on a boundary of so many bytes (null ones are)
+template <typename... P>
+inline bool on_boundary(size_t bytes, P... p) {
+    return ((reinterpret_cast<uintptr_t>(p) % bytes == 0) && ...);
+}
 inline int block_elem_size(int dtype) { return dtype == B200_F32 ? 4 : dtype == B200_BF16 || dtype == B200_F16 ? 2 : 0; }
 
 }  // namespace b200

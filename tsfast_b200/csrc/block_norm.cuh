@@ -379,7 +379,11 @@ inline int check(const Args& p, int dtype, int kind, bool res) {
     if (p.ldx < 0 || p.ldg < 0 || p.ldr < 0 || p.ldgy < 0 || p.ldgr < 0) return B200_ERR_ARG;
     if (!res && (p.par[kGScale] || !p.par[kGW1])) return B200_ERR_ARG;
     if (p.par[kGB1] && !p.par[kGW1]) return B200_ERR_ARG;
-    return B200_OK;
+    const int e = block_elem_size(dtype), f = p.pf32 ? 4 : e;
+    if (!on_boundary(e, p.x, p.gate, p.res, p.y, p.res_out, p.gy, p.gres, p.gx, p.ggate, p.gresid)) return B200_ERR_ARG;
+    for (const void* w : p.par)
+        if (!on_boundary(f, w)) return B200_ERR_ARG;
+    return on_boundary(16, p.stats) ? B200_OK : B200_ERR_ARG;
 }
 
 }  // namespace norm

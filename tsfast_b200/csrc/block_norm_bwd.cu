@@ -33,6 +33,7 @@ int b200_block_norm_bwd(int dtype, int64_t M, int64_t D, int kind, int act, floa
     if (rc != B200_OK) return rc;
     if (kind == 0 && (gb1 || gb2)) return B200_ERR_ARG;
     if ((gw1 && !w1) || (gb1 && !w1) || (gscale && !scale) || ((gw2 || gb2) && !res) || (ggate && !gate)) return B200_ERR_ARG;
+    if (!on_boundary(params_f32 ? 4 : block_elem_size(dtype), gw1, gb1, gscale, gw2, gb2) || !on_boundary(block_elem_size(dtype), ggate)) return B200_ERR_ARG;
     if (M > 0 && (!x || !gy || !stats || (res && (!residual || !gresidual)))) return B200_ERR_ARG;
     if (M > 0 && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < b200_block_norm_bwd_workspace_bytes(M, D, kind)))
         return B200_ERR_WORKSPACE;

@@ -1097,6 +1097,7 @@ int b200_gated_probe(int polls, int mute_step, int dtype, int64_t S, int64_t L, 
     const long long rows = packed ? T : S * L;
     if (S == 0 && rows == 0) return B200_OK;
     if (!lam || (S > 0 && !hlast) || (rows > 0 && (!x || !r || !i || !h))) return B200_ERR_ARG;
+    if (!on_boundary(4, lam, h0, hlast, chk) || !on_boundary(cu_is64 ? 8 : 4, cu)) return B200_ERR_ARG;
     Args p = {};
     p.in[0] = {x, xb, xt}, p.in[1] = {r, rb, rt}, p.in[2] = {i, ib, it};
     p.out[0] = h, p.lam = (const float*)lam, p.h0 = (const float*)h0, p.hlast = (float*)hlast, p.chk = (float*)chk;
@@ -1120,6 +1121,7 @@ int b200_gated_bwd(int dtype, int64_t S, int64_t L, int64_t T, int64_t D, float 
     const bool packed = cu != nullptr;
     const long long rows = packed ? T : S * L;
     if (!lam || !glam || (rows > 0 && (!x || !r || !i || !gh || !gx || !gr || !gi || !chk))) return B200_ERR_ARG;
+    if (!on_boundary(4, lam, chk, glast, glam, gh0) || !on_boundary(cu_is64 ? 8 : 4, cu)) return B200_ERR_ARG;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (S == 0 && rows == 0) return cudaMemsetAsync(glam, 0, (size_t)D * 4, st) == cudaSuccess ? B200_OK : B200_ERR_LAUNCH;
     const Workspace w = plan(dtype, S, L, T, (int)D, packed);
@@ -1147,6 +1149,7 @@ int b200_gated_step(int dtype, int64_t B, int64_t D, int64_t n, float c, const v
     if (e == 0 || B < 0 || n < 0 || D < 1 || D > (1 << 24) || state_pitch < D) return B200_ERR_ARG;
     if (B == 0) return B200_OK;
     if (!x || !r || !i || !lam || !h || (n > 0 && !state) || (!slots && n < B)) return B200_ERR_ARG;
+    if (!on_boundary(e, h) || !on_boundary(4, lam, state) || !on_boundary(slots_are64 ? 8 : 4, slots)) return B200_ERR_ARG;
     if (B > 65535) return B200_ERR_UNSUPPORTED;
     StepArgs p = {};
     p.in[0] = {x, xb, 0}, p.in[1] = {r, rb, 0}, p.in[2] = {i, ib, 0};

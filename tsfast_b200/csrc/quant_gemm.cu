@@ -683,6 +683,7 @@ int b200_quant_weight(int dtype, int64_t N, int64_t K, const void* w, int64_t ld
     using namespace b200;
     using namespace b200::quant;
     if (block_elem_size(dtype) == 0 || N < 1 || K < 1 || N > (1 << 22) || K > (1 << 22) || !w || !q || !scale || ldw < 0 || ldq < K) return B200_ERR_ARG;
+    if (!on_boundary(block_elem_size(dtype), w) || !on_boundary(4, scale)) return B200_ERR_ARG;
     const dim3 grid((unsigned int)((K + kBlock - 1) / kBlock), (unsigned int)((N + kBlock - 1) / kBlock));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == B200_F32) quant_weight_kernel<float><<<grid, 256, 0, st>>>((const float*)w, ldw, (int)N, (int)K, (uint8_t*)q, ldq, (float*)scale);
@@ -704,6 +705,7 @@ int b200_quant_probe(int polls, int64_t mute_tile, int dtype, int64_t M, int64_t
     if ((dtype != B200_BF16 && dtype != B200_F16) || M < 0 || N < 1 || K < 1 || N > (1 << 22) || K > (1 << 22) || M > 0x7fffff00LL) return B200_ERR_ARG;
     if (M == 0) return B200_OK;
     if (!x || !q || !scale || !y || ldx < 0 || ldy < N || ldq < K || ldq % 16 || (uintptr_t)q % 16 || (uintptr_t)x % 2 || (uintptr_t)y % 2) return B200_ERR_ARG;
+    if (!on_boundary(4, scale) || !on_boundary(bias_f32 ? 4 : 2, bias)) return B200_ERR_ARG;
     const Plan w = plan(M, N, K);
     if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < w.total) return B200_ERR_WORKSPACE;
     Args p = {};
