@@ -184,3 +184,29 @@ def test_c_entry_points_refuse_pointers_off_their_elements(built):
     assert lin(x=1) == lin(y=1) == lin(scale=2) == lin(bias=2) == lin(bias_f32=0, bias=1) == 1
     weight = lambda dtype=0, w=0, scale=0: L.b200_quant_weight(dtype, 4, 4, at(w), 4, at(), 4, at(scale), z)  # noqa: E731
     assert weight(w=2) == weight(dtype=2, w=1) == weight(scale=2) == 1
+
+
+def test_host_path_is_built_again_for_another_torch(built, monkeypatch, tmp_path):
+    import shutil
+
+    from tsfast_b200 import build
+
+    copy = tmp_path / build.HOST_LIB.name
+    shutil.copy2(build.HOST_LIB, copy)
+    monkeypatch.setattr(build, "HOST_LIB", copy)
+    runs = []
+
+    class Done:
+        returncode = 0
+
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **kw: runs.append(cmd) or Done)
+    assert build.host_is_current()
+    build.build_host()
+    assert not runs
+    monkeypatch.setattr(torch, "__version__", "2.0.0")
+    assert not build.host_is_current()
+    build.build_host()
+    assert len(runs) == 1 and any("torch 2.0.0" in a for a in runs[0])
+    monkeypatch.setattr(built, "_HOST", None)
+    with pytest.raises(RuntimeError, match="another torch"):
+        built.host()

@@ -137,9 +137,13 @@ def host():
     if _HOST is None:
         import importlib.util
 
-        path = _PKG / "lib" / "_block_host.so"
+        from . import build
+
+        path = build.HOST_LIB
         if not path.exists():
             raise RuntimeError(f"{path} not found: build it first with `python -m tsfast_b200.build`")
+        if not build.host_is_current():
+            raise RuntimeError(f"{path} was built for another torch or Python: build it again with `python -m tsfast_b200.build`")
         spec = importlib.util.spec_from_file_location("_block_host", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)

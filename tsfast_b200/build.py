@@ -83,6 +83,18 @@ def build(verbose: bool = False, force: bool = False, extra_flags: list[str] | N
     return out
 
 
+def host_tag() -> str:
+    """What the host path has to be built for; it stands in the built file."""
+    import torch
+
+    return f"b200 host path for torch {torch.__version__}, Python {sys.version_info.major}.{sys.version_info.minor}"
+
+
+def host_is_current() -> bool:
+    """Whether the built host path belongs to this torch and this Python."""
+    return HOST_LIB.exists() and host_tag().encode() + b"\0" in HOST_LIB.read_bytes()
+
+
 def build_host(force: bool = False) -> Path:
     """Compile the block operators' host path (a PyTorch extension module in C++, no CUDA code) with g++; returns its path."""
     import sysconfig
@@ -90,12 +102,13 @@ def build_host(force: bool = False) -> Path:
     import torch
 
     LIBDIR.mkdir(exist_ok=True)
-    if not force and not _stale(HOST_LIB, [HOST_SRC, INCLUDE / "b200scan.h"]):
+    if not force and host_is_current() and not _stale(HOST_LIB, [HOST_SRC, INCLUDE / "b200scan.h"]):
         return HOST_LIB
     root = Path(torch.__file__).resolve().parent
     cuda = Path(_nvcc()).resolve().parent.parent
     cmd = ["/usr/bin/g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_block_host",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DB200_HOST_TAG="{host_tag()}"']
     for inc in (root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include"):
         cmd += ["-isystem", str(inc)]
     cmd += ["-I" + sysconfig.get_paths()["include"], str(HOST_SRC), "-o", str(HOST_LIB), "-L" + str(root / "lib"), "-lc10", "-lc10_cuda",

@@ -17,6 +17,9 @@
 
 #include "../../../include/b200scan.h"
 
+// the torch and the Python that this is built for: looked for in the built file, which may not load with others
+extern "C" __attribute__((used, visibility("default"))) const char b200_host_tag[] = B200_HOST_TAG;
+
 namespace {
 
 using at::Tensor;
