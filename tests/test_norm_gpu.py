@@ -243,3 +243,26 @@ def test_opcheck_and_compile():
     eager = torch.autograd.grad(seam(*args), args)
     compiled = torch.autograd.grad(torch.compile(seam, fullgraph=True, backend="aot_eager")(*args), args)
     assert all(torch.equal(p, q) for p, q in zip(eager, compiled))
+
+
+@pytest.mark.parametrize("activation", ["sigmoid", "silu"])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [24, 200, 1003])
+def test_gradient_of_a_gate_at_every_opening(width, dt, activation):
+    """Value by value: the gate's gradient has the logistic function's slope s (1 - s), whose second factor goes to nothing where the gate is
+    open. u = 2^-24; s and 1 - s, the function of the other sign, are each within 1.5 |g| u and 8 u, the norm and the products
+    within 32 u; SiLU's slope s + g s (1 - s) adds terms of up to |g|."""
+    import tsfast_b200 as b
+
+    g = torch.tensor([-60.0, -20, -12, -8, -2, 0, 2, 5, 8, 10, 12, 14, 15, 16, 18, 20, 40, 60], device="cuda")
+    gate = g.to(dt)[:, None].expand(-1, width).contiguous().requires_grad_()
+    x = (torch.rand(len(g), width, device="cuda", generator=torch.Generator(device="cuda").manual_seed(width)) + 0.5).to(dt)
+    w, up = torch.ones(width, device="cuda", dtype=dt), torch.ones_like(x)
+    (got,) = torch.autograd.grad(b.gated_norm(x, gate, w, activation=activation), gate, up)
+    v, x64 = gate.detach().double(), x.double()
+    s, shut = torch.sigmoid(v), torch.sigmoid(-v)
+    slope = s * shut if activation == "sigmoid" else s * (1 + v * shut)
+    want = x64 / torch.sqrt(x64.square().mean(-1, keepdim=True) + 1e-6) * slope
+    rel = (4 * v.abs() + 64) * 2.0**-24 + (0 if dt == torch.float32 else torch.finfo(dt).eps / 2 * (1 + 2.0**-7))
+    err = (got.double() - want).abs() / (rel * want.abs())
+    assert (err <= 1).all(), f"gate {v.flatten()[err.argmax()]}: {got.flatten()[err.argmax()]} for {want.flatten()[err.argmax()]}"

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : 512, WARP ? 4 : 1) norm_
                 load_columns<T, E, AL>(c, src, row * pitch, v);
             }
         };
-        // n = w1 hat1 + b1 (or x), the gate's sigmoid and value, m = n value
+        // n = w1 hat1 + b1 (or x), the gate's sigmoid (without SiLU: it minus one) and value, m = n value
         float2 hat1[H], n[H], sig[H], val[H], gm[H], v[H];
         read(0, p.x, p.ldx, n);
         if constexpr (POST) {
@@ -121,6 +121,8 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : 512, WARP ? 4 : 1) norm_
             for (int j = 0; j < H; ++j) {
                 sig[j] = sigmoid_of(v[j]);
                 val[j] = silu ? mul2(sig[j], v[j]) : sig[j];
+                // the slope s (1 - s) of an open gate: 1 - s is the function of -v, the difference keeps nothing of it
+                if (!silu) sig[j] = neg2(sigmoid_of(neg2(v[j])));
             }
         } else {
 #pragma unroll
@@ -157,8 +159,8 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : 512, WARP ? 4 : 1) norm_
         if (gated) {
 #pragma unroll
             for (int j = 0; j < H; ++j) {
-                // SiLU: g s (1 - s) + s; the logistic function: s (1 - s)
-                const float2 slope = fma2(neg2(val[j]), sig[j], silu ? add2(val[j], sig[j]) : val[j]);
+                // SiLU: g s (1 - s) + s; the logistic function: s (1 - s), with s - 1 in `sig`
+                const float2 slope = fma2(neg2(val[j]), sig[j], silu ? add2(val[j], sig[j]) : both(0.f));
                 n[j] = mul2(mul2(gm[j], n[j]), slope);
                 gm[j] = mul2(gm[j], val[j]);
             }
