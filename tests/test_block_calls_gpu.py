@@ -250,3 +250,32 @@ def test_compiled_calls_refuse_what_eager_ones_refuse():
             compiled(lambda x, lam, h: b.gated_recurrence(x, x, x, lam, h))(wide, lam, torch.zeros(1, 2, 24, device="cuda"))
         h, last = compiled(lambda x, lam: b.gated_recurrence(x, x, x, lam))(wide[:, :, :0], lam)
         assert h.shape == (2, 1, 0, 24) and (last == 0).all()
+
+
+def checkpointed(f, *leaves):
+    from torch.utils.checkpoint import checkpoint
+
+    out = checkpoint(f, *leaves, use_reentrant=False)
+    return torch.autograd.grad(sum(o.square().sum() for o in flat(out)), leaves, allow_unused=True, materialize_grads=True)
+
+
+@pytest.mark.parametrize("name", ["recurrence", "recurrence 4-d", "recurrence packed", "gated_norm", "residual_norm"])
+def test_checkpointed_calls(name):
+    """Recomputation ends with an exception from inside the last operator that keeps a tensor: it has to come through as it is."""
+    f = calls()[name]
+    leaves = [t.requires_grad_() for t in tensors()]
+    want = torch.autograd.grad(sum(o.square().sum() for o in flat(f(*leaves))), leaves, allow_unused=True, materialize_grads=True)
+    assert all(torch.equal(a, w) for a, w in zip(checkpointed(f, *leaves), want, strict=True))
+
+
+@pytest.mark.parametrize("name", ["recurrence", "gated_norm", "residual_norm"])
+def test_an_exception_of_a_hook_keeps_its_type(name):
+    class Mine(Exception):
+        pass
+
+    def pack(t):
+        raise Mine("from the hook")
+
+    f, leaves = calls()[name], [t.requires_grad_() for t in tensors()]
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t), pytest.raises(Mine, match="from the hook"):
+        f(*leaves)

@@ -275,3 +275,24 @@ def test_error_words_read_zero():
         b.check_status()
     finally:
         b.track_status(False)
+
+
+def test_quantised_block_against_what_the_bits_stand_for():
+    """Both projections of the 8-bit block, each against float64 products of the quantised rows that go in and the weights that the
+    bits stand for: the second's rows are what the recurrence and the gated norm made of the first's results."""
+    import tsfast_b200 as b
+    from test_quant_gpu import check
+
+    D, N = 256, 384
+    layers, rand = weights(D, N, torch.bfloat16, seed=2, layers=1)
+    w = layers[0]
+    x = rand(50, D).bfloat16()
+    with torch.no_grad():
+        q_in, q_out = b.quantize_weight(w["in"]), b.quantize_weight(w["out"])
+        y, _ = b.residual_norm(x, x, w["norm"])
+        mixed = b.quant_linear(y, *q_in)
+        u, a, i, z = mixed.split(N, dim=-1)
+        h, _ = b.gated_recurrence(u, a, i, w["lam"], cu_seqlens=torch.tensor([0, 20, 50], device="cuda"))
+        inner = b.gated_norm(h, z, w["gated"])
+        check(y, *q_in, None, mixed)
+        check(inner, *q_out, None, b.quant_linear(inner, *q_out))
