@@ -328,10 +328,10 @@ int64_t b200_gated_chk_rows(int dtype, int64_t S, int64_t L, int64_t T, int pack
 int b200_gated_fwd(int dtype, int64_t S, int64_t L, int64_t T, int64_t D, float c, const void* cu, int cu_is64,
                    const void* x, int64_t xb, int64_t xt, const void* r, int64_t rb, int64_t rt, const void* i, int64_t ib,
                    int64_t it, const void* lam, const void* h0, void* h, void* hlast, void* chk, void* stream);
-/* Test probe: the same call with the polls that a wait makes before it gives up (0 = the default, about a second) and a
- * step (a tile per CTA of a chain; -1 = none) whose result the chain's first CTA keeps to itself, so that the waits for
- * it run out, the launch returns and b200_block_status reports B200_ERR_TIMEOUT. */
-int b200_gated_probe(int polls, int mute_step, int dtype, int64_t S, int64_t L, int64_t T, int64_t D, float c, const void* cu,
+/* Test probe: the same call with a step (a tile per CTA of a chain; -1 = none) with which the chain's first CTA falls silent, so
+ * that the waits for it run out (after about a second), the launch returns and b200_block_status reports
+ * B200_ERR_TIMEOUT. */
+int b200_gated_probe(int mute_step, int dtype, int64_t S, int64_t L, int64_t T, int64_t D, float c, const void* cu,
                      int cu_is64, const void* x, int64_t xb, int64_t xt, const void* r, int64_t rb, int64_t rt, const void* i,
                      int64_t ib, int64_t it, const void* lam, const void* h0, void* h, void* hlast, void* chk, void* stream);
 size_t b200_gated_bwd_workspace_bytes(int dtype, int64_t S, int64_t L, int64_t T, int64_t D, int packed);

@@ -175,14 +175,14 @@ def test_a_wait_that_runs_out_is_reported(dt, S, L, D, mute):
     assert lib.b200_block_status(stream) == 0
     tag = {torch.float32: 0, torch.bfloat16: 2}[dt]
 
-    def probe(mute, polls):
+    def probe(mute):
         h, end = torch.zeros_like(want), torch.zeros_like(last)
-        assert lib.b200_gated_probe(polls, mute, tag, S, L, 0, D, 8.0, None, 0, *(a for t in (x, r, i) for a in (_lib.ptr(t), L * D, D)), _lib.ptr(lam),
+        assert lib.b200_gated_probe(mute, tag, S, L, 0, D, 8.0, None, 0, *(a for t in (x, r, i) for a in (_lib.ptr(t), L * D, D)), _lib.ptr(lam),
                                     None, _lib.ptr(h), _lib.ptr(end), None, stream) == 0
         return h, end
 
-    assert all(torch.equal(a, w) for a, w in zip(probe(-1, 0), (want, last))) and lib.b200_block_status(stream) == 0
-    h, _ = probe(mute, 64)
+    assert all(torch.equal(a, w) for a, w in zip(probe(-1), (want, last))) and lib.b200_block_status(stream) == 0
+    h, _ = probe(mute)
     assert lib.b200_block_status(stream) == 5  # B200_ERR_TIMEOUT
     assert lib.b200_block_status(stream) == 0
     assert torch.equal(h[:, : 28 * mute], want[:, : 28 * mute])  # (later values are whatever shared memory held: the last call's, even)

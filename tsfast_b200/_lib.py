@@ -70,7 +70,7 @@ SIGNATURES = {
     "b200_block_status": (_int, [_vp]),
     "b200_gated_chk_rows": (_i64, [_int, _i64, _i64, _i64, _int]),
     "b200_gated_fwd": (_int, [_int] + [_i64] * 4 + [_f32, _vp, _int] + [_vp, _i64, _i64] * 3 + [_vp] * 6),
-    "b200_gated_probe": (_int, [_int, _int, _int] + [_i64] * 4 + [_f32, _vp, _int] + [_vp, _i64, _i64] * 3 + [_vp] * 6),
+    "b200_gated_probe": (_int, [_int, _int] + [_i64] * 4 + [_f32, _vp, _int] + [_vp, _i64, _i64] * 3 + [_vp] * 6),
     "b200_gated_bwd_workspace_bytes": (_sz, [_int] + [_i64] * 4 + [_int]),
     "b200_gated_bwd": (_int, [_int] + [_i64] * 4 + [_f32, _vp, _int] + [_vp, _i64, _i64] * 3 + [_vp, _vp]
                        + [_vp, _i64, _i64] + [_vp] * 7 + [_sz, _vp]),

@@ -218,7 +218,7 @@ struct Args {
     int ctiles, C;
     float c;
     int whole;          // outputs: rows of whole lanes of channels on an aligned base
-    int polls, mute;    // forward: polls of a wait; a step whose result the first CTA of every chain keeps to itself (-1: none)
+    int until;          // forward: the step with which the first CTA of every chain falls silent (the probe's; else past the last)
 };
 
 __device__ __forceinline__ long long boundary(const Args& p, long long k) {
@@ -356,8 +356,8 @@ __device__ __forceinline__ void arrive(uint64_t* bar) {
 // Bounded wait (a poll waits 4 us itself). One that runs out is remembered in `lost`: later waits return at once, the results are
 // wrong, and the error word says so.
 constexpr int kWaitLimit = 1 << 18;  // polls: about a second
-__device__ __forceinline__ void await(uint64_t* bar, uint32_t parity, int polls, bool& lost) {
-    for (int i = 0; i < polls && !lost; ++i) {
+__device__ __forceinline__ void await(uint64_t* bar, uint32_t parity, bool& lost) {
+    for (int i = 0; i < kWaitLimit && !lost; ++i) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -402,20 +402,18 @@ __device__ __forceinline__ void close_exchange(int C, bool lost) {
 }
 // The folding warp of every CTA tells all CTAs of its cluster its tile's maps, and folds theirs from the carry: the states
 // that enter this CTA's tile (in `enter`); the carry becomes those behind the last CTA's.
-// A lane that has lost a wait sends and expects nothing any more (the barrier would be arrived at twice in one phase), so all
-// CTAs lose theirs.
+// A lane that has lost a wait sends and expects nothing any more (`to` becomes zero; it is C before): the barrier would be
+// arrived at twice in one phase. So all CTAs lose theirs.
 template <int NP>
 __device__ __forceinline__ void exchange(Map (*peers)[NP][32], Barriers& b, int C, int rank, int s, const Map (&mine)[NP], Pair (&enter)[NP],
-                                         Pair (&carry)[NP], int polls, int mute, bool& lost) {
+                                         Pair (&carry)[NP], int& to, bool& lost) {
     const int buf = s & 1, lane = threadIdx.x & 31;
-    if (!lost) {
-        if (lane == 0) expect(&b.peers[buf], C * 32 * NP * (int)sizeof(Map));
-        if (s != mute || rank != 0)
-            for (int c = 0; c < C; ++c)
+    if (lane == 0 && to > 0) expect(&b.peers[buf], C * 32 * NP * (int)sizeof(Map));
+    for (int c = 0; c < to; ++c)
 #pragma unroll
-                for (int k = 0; k < NP; ++k) put_remote(&peers[buf * C + rank][k][lane], &b.peers[buf], c, mine[k]);
-        await(&b.peers[buf], (uint32_t)(s >> 1) & 1u, polls, lost);
-    }
+        for (int k = 0; k < NP; ++k) put_remote(&peers[buf * C + rank][k][lane], &b.peers[buf], c, mine[k]);
+    await(&b.peers[buf], (uint32_t)(s >> 1) & 1u, lost);
+    if (lost) to = 0;
     for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
@@ -467,11 +465,13 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const Args p) {
 
     if (wid == kWarps) {
         // ---------------------------------------------------------------- the warp that folds
+        int to = C;
         Pair carry[NP] = {}, h[NP];
         if (p.h0 != nullptr) load_state<NP>(p.h0 + seq * p.D + d, n, carry);
-        for (int s = 0; s < steps; ++s) {
+        const int mine = rank == 0 ? min(steps, p.until) : steps;
+        for (int s = 0; s < mine; ++s) {
             const int buf = s & 1, tile = s * C + rank;
-            await(&bars.maps[buf], (uint32_t)(s >> 1) & 1u, p.polls, lost);
+            await(&bars.maps[buf], (uint32_t)(s >> 1) & 1u, lost);
             if (C == 1) {
 #pragma unroll
                 for (int k = 0; k < NP; ++k) h[k] = carry[k];
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const Args p) {
 #pragma unroll
                     for (int w = 1; w < kWarps; ++w) whole[k] = after(maps[buf][w][k][lane], whole[k]);
                 }
-                exchange<NP>(peers, bars, C, rank, s, whole, h, carry, p.polls, p.mute, lost);
+                exchange<NP>(peers, bars, C, rank, s, whole, h, carry, to, lost);
             }
             if (p.chk != nullptr && tile < tiles) store_state<NP>(p.chk + (ch.slot0 + tile) * p.D + d, n, h);
 #pragma unroll
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const Args p) {
                 for (int k = 0; k < NP; ++k) carry[k] = h[k];
             }
             __syncwarp();
-            if (lane == 0 && (C > 1 || s != p.mute)) arrive(&bars.start[buf]);
+            if (lane == 0) arrive(&bars.start[buf]);
         }
         if (rank == 0) store_state<NP>(p.hlast + seq * p.D + d, n, carry);
     } else {
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const Args p) {
         auto states = [&](int s, const Pair(&a)[TS][NP], const Pair(&b)[TS][NP]) {
             const int row0 = (s * C + rank) * kTile + wid * TS, left = ch.len - row0;
             T* out = static_cast<T*>(p.out[0]) + (ch.row0 + row0) * p.D + d;
-            await(&bars.start[s & 1], (uint32_t)(s >> 1) & 1u, p.polls, lost);
+            await(&bars.start[s & 1], (uint32_t)(s >> 1) & 1u, lost);
             Pair h[NP];
 #pragma unroll
             for (int e = 0; e < NP; ++e) h[e] = start[s & 1][wid][e][lane];
@@ -628,6 +628,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
     open_exchange(C, bars);
 
     if (wid == kWarps) {
+        int to = C;
         Pair carry[NP] = {}, next[NP];
         if (p.glast != nullptr) load_state<NP>(p.glast + seq * p.D + d, n, carry);
         auto kept = [&](int s) {
@@ -643,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
 #pragma unroll
             for (int k = 0; k < NP; ++k) h[k] = next[k];
             kept(s + 1);
-            await(&bars.maps[buf], (uint32_t)(s >> 1) & 1u, kWaitLimit, lost);
+            await(&bars.maps[buf], (uint32_t)(s >> 1) & 1u, lost);
             if (C == 1) {
 #pragma unroll
                 for (int k = 0; k < NP; ++k) g[k] = carry[k];
@@ -655,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
 #pragma unroll
                     for (int w = kWarps - 2; w >= 0; --w) whole[k] = after(maps[buf][w][k][lane], whole[k]);
                 }
-                exchange<NP>(peers, bars, C, rank, s, whole, g, carry, kWaitLimit, -1, lost);
+                exchange<NP>(peers, bars, C, rank, s, whole, g, carry, to, lost);
             }
 #pragma unroll
             for (int k = 0; k < NP; ++k) {
@@ -763,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
         };
         auto gradients = [&](int s, const Coeffs& f) {
             const int row0 = first_row(s), left = row0 < 0 ? 0 : ch.len - row0;
-            await(&bars.start[s & 1], (uint32_t)(s >> 1) & 1u, kWaitLimit, lost);
+            await(&bars.start[s & 1], (uint32_t)(s >> 1) & 1u, lost);
             Pair g[NP], before[TS][NP], x[NP];
 #pragma unroll
             for (int e = 0; e < NP; ++e) {
@@ -1084,10 +1085,10 @@ int64_t b200_gated_chk_rows(int dtype, int64_t S, int64_t L, int64_t T, int pack
 int b200_gated_fwd(int dtype, int64_t S, int64_t L, int64_t T, int64_t D, float c, const void* cu, int cu_is64, const void* x, int64_t xb,
                    int64_t xt, const void* r, int64_t rb, int64_t rt, const void* i, int64_t ib, int64_t it, const void* lam, const void* h0,
                    void* h, void* hlast, void* chk, void* stream) {
-    return b200_gated_probe(0, -1, dtype, S, L, T, D, c, cu, cu_is64, x, xb, xt, r, rb, rt, i, ib, it, lam, h0, h, hlast, chk, stream);
+    return b200_gated_probe(-1, dtype, S, L, T, D, c, cu, cu_is64, x, xb, xt, r, rb, rt, i, ib, it, lam, h0, h, hlast, chk, stream);
 }
 
-int b200_gated_probe(int polls, int mute_step, int dtype, int64_t S, int64_t L, int64_t T, int64_t D, float c, const void* cu, int cu_is64, const void* x,
+int b200_gated_probe(int mute_step, int dtype, int64_t S, int64_t L, int64_t T, int64_t D, float c, const void* cu, int cu_is64, const void* x,
                      int64_t xb, int64_t xt, const void* r, int64_t rb, int64_t rt, const void* i, int64_t ib, int64_t it, const void* lam,
                      const void* h0, void* h, void* hlast, void* chk, void* stream) {
     using namespace b200;
@@ -1102,7 +1103,7 @@ int b200_gated_probe(int polls, int mute_step, int dtype, int64_t S, int64_t L, 
     p.in[0] = {x, xb, xt}, p.in[1] = {r, rb, rt}, p.in[2] = {i, ib, it};
     p.out[0] = h, p.lam = (const float*)lam, p.h0 = (const float*)h0, p.hlast = (float*)hlast, p.chk = (float*)chk;
     p.cu = cu, p.cu64 = cu_is64, p.S = S, p.L = L, p.T = T, p.D = (int)D, p.c = c;
-    p.polls = polls > 0 && polls < kWaitLimit ? polls : kWaitLimit, p.mute = mute_step;
+    p.until = mute_step < 0 ? 0x7fffffff : mute_step;
     return dispatch(dtype, false, p, S, rows, static_cast<cudaStream_t>(stream));
 }
 
