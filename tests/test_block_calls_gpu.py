@@ -279,3 +279,16 @@ def test_an_exception_of_a_hook_keeps_its_type(name):
     f, leaves = calls()[name], [t.requires_grad_() for t in tensors()]
     with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t), pytest.raises(Mine, match="from the hook"):
         f(*leaves)
+
+
+def test_a_compiled_program_quantises_its_weight():
+    import tsfast_b200 as b
+
+    def f(w, x):
+        q, scale = b.quantize_weight(w)
+        return b.quant_linear(x, q, scale), q.float(), scale
+
+    w, x = torch.randn(150, 200, device="cuda"), torch.randn(9, 200, device="cuda").bfloat16()
+    with torch.no_grad():
+        for a, want in zip(torch.compile(f, fullgraph=True, backend="aot_eager")(w, x), f(w, x), strict=True):
+            assert torch.equal(a, want)
