@@ -321,6 +321,7 @@ int b200_block_status(void* stream);
  * h, gx, gr, gi are dense rows of D.  h0 NULL: zero start.  hlast [S,D] is written always.  chk NULL or
  * float32 [b200_gated_chk_rows, D]: the states that enter each tile, which the adjoint takes instead of
  * h.  Backward: gh upstream gradient, glast [S,D] that of hlast (NULL: zero); gh0 NULL: not wanted.
+ * Pointers are on their elements' boundaries (else B200_ERR_ARG, here and in the entries below).
  * Sums go through the workspace in a fixed order.  Rows that do not start on 16-byte boundaries are
  * fetched in whole 16-byte granules: the granule of a row's first element may begin up to 14 bytes before it.
  * L and T are below 2^30. */
@@ -376,7 +377,8 @@ int b200_block_norm_bwd(int dtype, int64_t M, int64_t D, int kind, int act, floa
 /* ---- Product in 8-bit floating point with a scale per block of 128 ---------------------------------
  * y[m,n] = sum_k x'[m,k] w'[n,k] (+ bias[n]), x' and w' the values that x and w stand for in e4m3 with
  * power-of-two scales: the smallest power of two s with |v| <= 448 s (1 for zeros, never below 2^-126), one per
- * row and 128 consecutive k of x, one per 128 x 128 block of w.  Values that are not finite become NaN.
+ * row and 128 consecutive k of x, one per 128 x 128 block of w.  Values that are not finite become NaN (those of w set
+ * no scale; of x, the row's results are NaN).
  * b200_quant_weight: w [N,K] (B200_F32, B200_BF16 or B200_F16, row pitch ldw) -> q e4m3 [N,K] with row pitch
  * ldq, scale float32 [ceil(N/128), ceil(K/128)].  b200_quant_linear: x [M,K] and y [M,N] B200_BF16 or B200_F16
  * with row pitches ldx, ldy; x is quantised into the workspace; q 16-byte aligned with ldq a multiple of 16,

@@ -25,12 +25,14 @@
 // time, and the folding warps pass the tiles' maps through distributed shared memory with st.async: no flags in global
 // memory, nothing to reset, a fixed order of every sum. All waits are bounded (b200_block_status reads the error word).
 //
-// Measured (bytes are the tensors once: 4 forward, 7 in the adjoint): 8 x 4096 x 2048 float32 215 us and 359 us, 5.0 and 5.2
-// TB/s, near what memory gives; bfloat16 157 and 310 us, 3.4 and 3.0 TB/s. In 16 bits it is the arithmetic that bounds them, not
-// memory: 40 and 69 instructions per pair of channels, issued in 0.51 and 0.44 of the cycles by the sixteen warps that the
+// Measured (bytes are the tensors once: 4 forward, 7 in the adjoint): 8 x 4096 x 2048 float32 217 us and 362 us, 4.9 and 5.2
+// TB/s, near what memory gives; bfloat16 153 and 332 us, 3.5 and 2.8 TB/s. In 16 bits it is the arithmetic that bounds them, not
+// memory: 39 and 74 instructions per channel and step, issued in 0.51 and 0.45 of the cycles by the sixteen warps that the
 // registers allow, the rest being latencies of the chain loads - gates - maps - states. A deeper ring does not help (adjoint:
-// 311 us with three stages and one copy of the maps, 307 with two; forward: 160 us with four stages, 156 with three).
-// One 65536 x 1024 prompt (bfloat16, clusters of twelve): 224 us forward.
+// 311 us with three stages and one copy of the maps, 307 with two; forward: 160 us with four stages, 156 with three). Decays below
+// 2^-1/2 take the longer form of the exponential: 173 and 354 us. The adjoint's 1 - rho and 1 - iota cost it a second exponential
+// each, and a reciprocal (312 us with the differences, which lose their digits at open gates).
+// One 65536 x 1024 prompt (bfloat16, clusters of twelve): 226 us forward.
 #include "block.cuh"
 
 namespace b200 {
@@ -600,7 +602,8 @@ __global__ void __launch_bounds__(kThreads, 2) gated_fwd_kernel(const Args p) {
 // ------------------------------------------------------------------------------------------- adjoint
 // Tiles from the last to the first; CTA `rank` of a cluster takes the tile `rank` places before the newest. Inside a
 // tile the states run forward from the kept state and the adjoint runs backward from the carry; both folds use the
-// same products of decays, so one exchange of (A, forward sum, backward sum) serves both.
+// same products of decays, so a segment hands over one decay and two sums. Between CTAs only the adjoint's maps travel: every tile
+// has its own kept state.
 template <typename T, bool MIS, int NP>
 __global__ void __launch_bounds__(kThreads, 2) gated_bwd_kernel(const Args p) {
     using R = Rows<T, MIS, NP, true>;
@@ -973,8 +976,8 @@ __global__ void __launch_bounds__(kStepThreads) gated_step_kernel(const StepArgs
 }
 
 // ------------------------------------------------------------------------------------------- host
-// How a call is cut up: pairs of channels per lane, chains of a sequence, CTAs per chain. Two CTAs fit on an SM, and one
-// round of them is best: the largest of 1, 2, 4, 8 and 12 CTAs per chain that stays within 2 x 148 (8 x 4096 x 2048 bf16, 128
+// How a call is cut up: pairs of channels per lane, chains of a sequence, CTAs per chain. Two CTAs fit on an SM (but for the adjoint
+// of 16 bits with two pairs per lane and clusters of twelve, 118 KB each: one), and one round of them is best: the largest of 1, 2, 4, 8 and 12 CTAs per chain that stays within 2 x 148 (8 x 4096 x 2048 bf16, 128
 // chains, forward and adjoint: 595 us with one, 473 with two, 530 with three, 489 with four; 65536 x 1024, 16 chains: 1010
 // with eight, 722 with twelve, 947 with sixteen, which few GPCs can hold twice). Packed sequences differ in length, and several
 // rounds even them out (23 of 0 to 3000 steps, 368 chains: 349 us with one CTA, 239 with four). Chains in 16 bits are 128

@@ -22,8 +22,9 @@
 //            in the result's type, give it back and store while the next tile is under way
 // Many tokens: a pair of CTAs (cta_group::2) makes 256 features x 256 tokens, and each fetches half of either operand, 33 KB
 // per block instead of 49, six of them on their way. One CTA per tile is bound by what it fetches: 258 us at 8192 x 8192 x 4096
-// against 221 (2480 TFLOP/s with the quantisation of x; 200 of them remain if x is not fetched, and 181 without any fetching or storing,
-// close to the 4 x 128 cycles of a block's MMAs). What issues the MMAs is one elected lane: a lane chosen by its number makes
+// against 221 (2480 TFLOP/s with the quantisation of x, calls one by one; 266 to 284 us, about 2000 TFLOP/s, in a long run of them, where
+// the clock falls under the power limit; 200 us remain if x is not fetched, and 181 without any fetching or storing, close to the
+// 4 x 128 cycles of a block's MMAs). What issues the MMAs is one elected lane: a lane chosen by its number makes
 // the compiler loop over lanes for every instruction, and 263 us.
 // Few tiles (small M): a cluster of S CTAs shares a tile, each with its part of K; the parts meet in distributed shared
 // memory and are added in the order of the ranks. Every wait on an mbarrier is bounded: one that runs out raises a

@@ -6,7 +6,8 @@ Per channel, with ``rho = sigmoid(r_t)``, ``iota = sigmoid(i_t)`` and ``a_t = ex
 
 ``selective_recurrence`` takes a ready ``a_t`` and float32 sequences; here the gates' pre-activations go in as the
 projections leave them (float32, bfloat16 or float16, slices of one product's output are read in place), the state is
-float32 whatever the sequences' type, and sequences may be packed end to end.
+float32 whatever the sequences' type, and sequences may be packed end to end.  The first step of a sequence is like the others:
+its input too has the factor ``sqrt(1 - a_t^2)`` (some released models of this recurrence use one there).
 
 * ``gated_recurrence(x, r, i, lam, h0=None, cu_seqlens=None, c=8.0)`` -> ``(h, h_last)``, differentiable in ``x``,
   ``r``, ``i``, ``lam`` and ``h0``;
@@ -90,7 +91,8 @@ def gated_recurrence(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, lam: tor
 
     With ``cu_seqlens`` (int32 or int64 ``[S + 1]`` on the device, non-decreasing) ``x`` is ``[T, D]`` and sequence ``s``
     is rows ``cu_seqlens[s]`` to ``cu_seqlens[s + 1] - 1`` with its own ``h0[s]`` and ``h_last[s]``; sequences may be empty,
-    and rows before the first and behind the last get zeros, in ``h`` and in the gradients.
+    and rows before the first and behind the last get zeros, in ``h`` and in the gradients.  First derivatives backward only: second
+    ones, forward-mode ones and the transforms of ``torch.func`` raise.  ``h0`` is not kept for the backward pass.
     """
     if not torch.compiler.is_compiling():
         out = _lib.host().gated_recurrence(x, r, i, lam, h0, cu_seqlens, c)
@@ -126,7 +128,7 @@ def gated_recurrence_step(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, lam
 
     ``slots`` (int32 or int64 ``[B]`` on the device) names each row's state; without it row b has state b.  A slot
     outside the cache (-1 for an empty row of a padded batch) leaves the cache alone and its row of ``h`` is zeros; rows
-    that name the same slot are applied in row order.  There is no gradient: train with ``gated_recurrence``.
+    that name the same slot are applied in row order.  Up to 65535 rows.  There is no gradient: train with ``gated_recurrence``.
     """
     if not torch.compiler.is_compiling():
         out = _lib.host().gated_recurrence_step(x, r, i, lam, state, slots, c)

@@ -23,7 +23,8 @@ __all__ = ["quantize_weight", "quant_linear"]
 
 def quantize_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(q, scale)`` of a weight ``[N, K]`` (float32, bfloat16 or float16): ``q`` float8_e4m3fn ``[N, K]`` with a row pitch
-    that is a multiple of 128, ``scale`` float32 ``[ceil(N / 128), ceil(K / 128)]``.  A value that is not finite becomes NaN."""
+    that is a multiple of 128, ``scale`` float32 ``[ceil(N / 128), ceil(K / 128)]``.  A value that is not finite becomes NaN and sets no scale:
+    the others of its block are quantised as without it."""
     if not torch.compiler.is_compiling():
         out = _lib.host().quantize_weight(w)
         if out is not None:
