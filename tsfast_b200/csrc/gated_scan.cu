@@ -976,12 +976,13 @@ __global__ void __launch_bounds__(kStepThreads) gated_step_kernel(const StepArgs
 }
 
 // ------------------------------------------------------------------------------------------- host
-// How a call is cut up: pairs of channels per lane, chains of a sequence, CTAs per chain. Two CTAs fit on an SM (but for the adjoint
-// of 16 bits with two pairs per lane and clusters of twelve, 118 KB each: one), and one round of them is best: the largest of 1, 2, 4, 8 and 12 CTAs per chain that stays within 2 x 148 (8 x 4096 x 2048 bf16, 128
-// chains, forward and adjoint: 595 us with one, 473 with two, 530 with three, 489 with four; 65536 x 1024, 16 chains: 1010
-// with eight, 722 with twelve, 947 with sixteen, which few GPCs can hold twice). Packed sequences differ in length, and several
-// rounds even them out (23 of 0 to 3000 steps, 368 chains: 349 us with one CTA, 239 with four). Chains in 16 bits are 128
-// channels wide (10 x 1500 x 700: 144 us against 170 with 64), or 64 where those would be too few.
+// How a call is cut up: pairs of channels per lane, chains of a sequence, CTAs per chain. Two CTAs fit on an SM (but for the
+// adjoint of 16 bits with two pairs per lane and clusters of twelve, 118 KB each: one), and one round of them is best: the
+// largest of 1, 2, 4, 8 and 12 CTAs per chain that stays within 2 x 148 (8 x 4096 x 2048 bf16, 128 chains, forward and adjoint: 595 us
+// with one, 473 with two, 530 with three, 489 with four; 65536 x 1024, 16 chains: 1010 with eight, 722 with twelve, 947 with sixteen,
+// which few GPCs can hold twice). Packed sequences differ in length, and several rounds even them out (23 of 0 to 3000 steps, 368
+// chains: 349 us with one CTA, 239 with four). Chains in 16 bits are 128 channels wide (10 x 1500 x 700: 144 us against 170 with 64),
+// or 64 where those would be too few.
 struct Cut {
     int np, ctiles, C;
 };
